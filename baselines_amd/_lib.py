@@ -18,6 +18,9 @@ UNIQUE_ID_BYTES = 128
 POLICY_MLP, POLICY_CNN, POLICY_CNN_LSTM, POLICY_CNN_LNLSTM = 0, 1, 2, 3
 DIST_GAUSSIAN, DIST_CATEGORICAL = 0, 1
 ORDER_FORK, ORDER_UPSTREAM = 0, 1
+F32, BF16, F16 = 0, 1, 2
+GLR_SPAN = 16
+ADAMW_BLOCK = 256
 
 
 class PolicyDesc(Structure):
@@ -34,6 +37,15 @@ class Rollout(Structure):
     _fields_ = [("obs", c_void_p), ("actions", c_void_p), ("returns", c_void_p), ("values", c_void_p),
                 ("neglogpacs", c_void_p), ("advs", c_void_p), ("masks", c_void_p), ("states", c_void_p),
                 ("adv_f64", c_int32), ("T", c_int32), ("E", c_int32), ("_pad", c_int32), ("n", c_int64)]
+
+
+class Seq(Structure):
+    _fields_ = [("data", c_void_p), ("t", c_int64), ("e", c_int64)]
+
+
+class AdamwTensor(Structure):
+    _fields_ = [("param", c_void_p), ("n", c_int64), ("param_dtype", c_int32), ("grad_dtype", c_int32), ("decay", c_float),
+                ("reserved", c_int32)]
 
 
 class Ppo2HipError(RuntimeError):
@@ -127,6 +139,20 @@ _SIGS = {
     "ppo2hip_ppo_epoch_shares": (c_int, [POINTER(PolicyDesc), POINTER(LossDesc), _P, _P, _P, _P, POINTER(Rollout), _P, c_int64,
                                          POINTER(c_int64), c_int, _P, c_float, c_double, c_double, c_int64, c_double, c_double,
                                          c_double, c_double, _P, _P, c_size_t, _P, c_void_p, _P]),
+    "ppo2hip_glr_saved_floats": (c_int64, [c_int, c_int, c_int]),
+    "ppo2hip_glr_forward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "ppo2hip_glr_forward": (c_int, [c_int, c_int, c_int, c_int, POINTER(Seq), POINTER(Seq), _P, POINTER(Seq), _P, POINTER(Seq), _P,
+                                    _P, _P, c_size_t, _P]),
+    "ppo2hip_glr_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "ppo2hip_glr_backward": (c_int, [c_int, c_int, c_int, c_int, POINTER(Seq), POINTER(Seq), _P, POINTER(Seq), _P, POINTER(Seq), _P,
+                                     POINTER(Seq), POINTER(Seq), _P, _P, _P, c_size_t, _P]),
+    "ppo2hip_adamw_state_elements": (c_int64, [POINTER(AdamwTensor), c_int, c_int]),
+    "ppo2hip_adamw_plan_bytes": (c_size_t, [POINTER(AdamwTensor), c_int]),
+    "ppo2hip_adamw_plan_fill": (c_int, [POINTER(AdamwTensor), c_int, c_int, _P, c_size_t]),
+    "ppo2hip_adamw_workspace_bytes": (c_size_t, [POINTER(AdamwTensor), c_int]),
+    "ppo2hip_adamw_step": (c_int, [POINTER(AdamwTensor), c_int, c_int, _P, POINTER(c_void_p), _P, _P, _P, _P, c_double, c_int64,
+                                   c_double, c_double, c_double, c_double, c_double, c_double, _P, _P, c_size_t, _P]),
+    "ppo2hip_adamw_state": (c_int, [POINTER(AdamwTensor), c_int, _P, _P, _P, _P, _P, c_int, _P, _P, _P]),
     "ppo2hip_gemm_f32": (c_int, [_P, _P, _P, c_int, c_int, c_int, _P]),
 }
 

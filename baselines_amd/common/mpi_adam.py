@@ -208,3 +208,56 @@ class MpiAdam:
 
     def check_synced(self):
         self.comm.check_synced(self.theta)
+
+
+class MpiAdamW:
+    """MpiAdam's role for a list of tensors and AdamW: ``update(grads, stepsize)`` checks the replicas every 100 calls
+    (mpi_adam.py:22-23), sums the gradients over the ranks, scales by 1/size (``scale_grad_by_procs``, :27-28), clips by the
+    global norm when ``max_grad_norm`` > 0 and steps every tensor in one kernel launch; ``sync`` broadcasts rank 0's
+    parameters (:37-40).  ``params``, ``decay``, ``state_bits`` (32, or 8 for moments in codes) and ``state`` are those of
+    ``hip.AdamWPlan``, held in ``self.plan``.
+
+    A gradient may be None (its tensor is left out of the step) in a single process only: ranks add one packed float32
+    buffer, so each of them has to bring every gradient."""
+
+    def __init__(self, params, *, beta1=0.9, beta2=0.999, epsilon=1e-08, weight_decay=0.01, decay=None, state_bits=32,
+                 max_grad_norm=0.0, scale_grad_by_procs=True, comm=None, state=None, grad_dtype=None):
+        from .. import hip
+        self._hip = hip
+        self.comm = comm or DataParallel("mpi")
+        self.beta1, self.beta2, self.epsilon, self.weight_decay = beta1, beta2, epsilon, weight_decay
+        self.max_grad_norm = max_grad_norm
+        self.scale_grad_by_procs = scale_grad_by_procs
+        self.params = list(params)
+        if self.comm.size > 1:
+            grad_dtype = torch.float32           # the type of the buffer that the ranks add up
+        self.plan = hip.AdamWPlan(self.params, state_bits=state_bits, decay=decay, state=state, grad_dtype=grad_dtype)
+        self.t = 0
+        self._sum = self._views = None
+        if self.comm.size > 1:
+            self._sum = torch.empty(self.plan.numel, dtype=torch.float32, device=self.plan.device)
+            self._views = [v.view(p.shape) for v, p in zip(self._sum.split([p.numel() for p in self.params]), self.params)]
+
+    def update(self, grads, stepsize):
+        if self.t % 100 == 0:
+            self.check_synced()
+        grads = list(grads)
+        if self.comm.size > 1:
+            if len(grads) != len(self._views) or any(g is None for g in grads):
+                raise ValueError("every rank must bring a gradient for each of the %d tensors" % len(self._views))
+            for v, g in zip(self._views, grads):
+                v.copy_(g)
+            self.comm.allreduce_sum_(self._sum)
+            grads = self._views
+        scale = 1.0 / self.comm.size if self.scale_grad_by_procs else 1.0
+        self._hip.adamw_step(self.plan, grads, stepsize, self.t + 1, beta1=self.beta1, beta2=self.beta2, epsilon=self.epsilon,
+                             weight_decay=self.weight_decay, max_grad_norm=self.max_grad_norm, grad_scale=scale)
+        self.t += 1
+
+    def sync(self):
+        for p in self.plan.params:
+            self.comm.bcast_(p)
+
+    def check_synced(self):
+        if self.comm.size > 1:
+            self.comm.check_synced(torch.cat([p.reshape(-1).float() for p in self.plan.params]))

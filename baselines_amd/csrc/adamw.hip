@@ -1,0 +1,452 @@
+// AdamW over a list of tensors in one launch (two when the gradients are clipped by their global norm), moments held in
+// float32 or in 8 bits per block of 256 elements:
+//   m = b1 m + (1 - b1) g    v = b2 v + (1 - b2) g^2    p -= lr (m / (1 - b1^t) / (sqrt(v / (1 - b2^t)) + eps) + wd p)
+//   8 bits: m = sm sign(c) (c / 127)^2,  v = sv (c / 255)^4, sm and sv the block's largest |m| and v.
+// The powers space the codes by a constant share of the square (fourth) root, so that a code's relative step is 2 / c
+// (4 / c): 1.6 % at the block's largest element, and v reaches down to 2^-32 of it, where even steps would round all
+// that is below 1/510 to zero and divide by epsilon alone.  A v that is not zero never gets code 0 for the same reason.
+#include <cmath>
+
+#include "kernels.hpp"
+
+namespace ppo2hip {
+
+constexpr int kBlock = PPO2HIP_ADAMW_BLOCK;      // elements of one scale
+constexpr int kChunk = 2048;                     // elements a workgroup takes at a time: 8 per thread, 8 blocks of 8-bit moments
+constexpr int kThreads = 256;
+constexpr int kMaxGrads = 448;                   // gradient pointers of one launch: they ride in its 4 KB of arguments
+constexpr int kNormGroups = 1024;                // workgroups of the norm launch = partial sums every workgroup of the step adds up
+
+struct TensorRow {                               // one tensor in the device image of a plan
+    void *p;
+    int64_t n;                                   // elements
+    int64_t off;                                 // first element in the moments
+    int32_t p_type, g_type;
+    float decay;
+    int32_t pad;
+};
+struct ChunkRow {
+    int32_t tensor, index;                       // chunk `index` of kChunk elements of that tensor
+};
+
+struct AdamwArgs {
+    const TensorRow *tensors;
+    const ChunkRow *chunks;
+    int32_t first_tensor, nchunks;               // of this launch
+    void *m, *v;
+    float *m_scale, *v_scale;
+    const double *partial;
+    int32_t npartial;
+    float lr, c1, c2, b1, b2, omb1, omb2, eps, wd, gscale, max_norm;
+    float *norm_out;
+    const void *g[kMaxGrads];
+};
+static_assert(sizeof(AdamwArgs) <= 4096, "arguments beyond what a launch carries");
+
+struct NormArgs {
+    const TensorRow *tensors;
+    const ChunkRow *chunks;
+    int32_t first_tensor, nchunks;
+    double *partial;
+    float gscale;
+    const void *g[kMaxGrads];
+};
+
+// four elements from any element-aligned address: one wide load where all four exist
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef f32x4 f32x4_any __attribute__((aligned(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef bf16x4 bf16x4_any __attribute__((aligned(2)));
+
+__device__ inline f32x4 load4(const void *base, int type, int64_t i, int64_t n) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (type == PPO2HIP_F32) {
+        const float *p = (const float *)base + i;
+        if (i + 4 <= n) return *(const f32x4_any *)p;
+        for (int k = 0; k < 3; k++)
+            if (i + k < n) r[k] = p[k];
+    } else {
+        const __bf16 *p = (const __bf16 *)base + i;
+        if (i + 4 <= n) return __builtin_convertvector(*(const bf16x4_any *)p, f32x4);
+        for (int k = 0; k < 3; k++)
+            if (i + k < n) r[k] = (float)p[k];
+    }
+    return r;
+}
+// a bfloat16 parameter is rounded to nearest: an update below half its step is lost, as in any bfloat16 weight without a
+// wider copy
+__device__ inline void store4(void *base, int type, int64_t i, int64_t n, f32x4 v) {
+    if (type == PPO2HIP_F32) {
+        float *p = (float *)base + i;
+        if (i + 4 <= n) *(f32x4_any *)p = v;
+        else
+            for (int k = 0; k < 3; k++)
+                if (i + k < n) p[k] = v[k];
+    } else {
+        __bf16 *p = (__bf16 *)base + i;
+        if (i + 4 <= n) *(bf16x4_any *)p = __builtin_convertvector(v, bf16x4);
+        else
+            for (int k = 0; k < 3; k++)
+                if (i + k < n) p[k] = (__bf16)v[k];
+    }
+}
+
+// The values codes stand for.  The integer powers are exact (a fourth power past 2^24 rounds once), so that what is raised
+// carries no rounding that the power would multiply.
+__device__ inline float moment_of(int8_t c, float scale) {
+    const float x = (float)c;
+    return scale * (x * fabsf(x) * (1.f / 16129.f));
+}
+__device__ inline float square_of(uint8_t c, float scale) {
+    const float x = (float)((unsigned)c * c);
+    return scale * (x * x * (1.f / 4228250625.f));
+}
+
+__global__ __launch_bounds__(kThreads) void adamw_norm_kernel(NormArgs a) {
+    __shared__ double red[17];
+    double s = 0.0;
+    for (int c = blockIdx.x; c < a.nchunks; c += gridDim.x) {
+        const ChunkRow ch = a.chunks[c];
+        const void *g = a.g[ch.tensor - a.first_tensor];
+        if (!g) continue;
+        const TensorRow &t = a.tensors[ch.tensor];
+#pragma unroll
+        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
+            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
+            if (i >= t.n) break;
+            const f32x4 x = load4(g, t.g_type, i, t.n);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const double d = (double)(x[k] * a.gscale);
+                s += d * d;                       // in 64 bits: squares of float32 leave its range
+            }
+        }
+    }
+    s = block_sum(s, red);
+    if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
+}
+
+__device__ inline unsigned wave_umax(unsigned v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        const unsigned w = (unsigned)__shfl_xor((int)v, o, 64);
+        v = v > w ? v : w;
+    }
+    return v;
+}
+
+template <int BITS>
+__global__ __launch_bounds__(kThreads) void adamw_kernel(AdamwArgs a) {
+    __shared__ double red[17];
+    float scale = a.gscale;
+    if (a.max_norm > 0.f) {
+        double s = 0.0;
+        for (int i = threadIdx.x; i < a.npartial; i += kThreads) s += a.partial[i];
+        s = block_sum(s, red);
+        const float norm = (float)sqrt(s);
+        // not fmaxf: a norm that is not a number stays one
+        scale = a.gscale * (norm > a.max_norm ? a.max_norm / norm : (norm <= a.max_norm ? 1.f : norm));
+        if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[0] = norm;
+    }
+    if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[1] = scale;
+
+    for (int c = blockIdx.x; c < a.nchunks; c += gridDim.x) {
+        const ChunkRow ch = a.chunks[c];
+        const void *gp = a.g[ch.tensor - a.first_tensor];
+        if (!gp) continue;
+        const TensorRow t = a.tensors[ch.tensor];
+        const float wd = a.wd * t.decay;
+#pragma unroll
+        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
+            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
+            if ((BITS == 32 ? i : i - (threadIdx.x & 63) * 4) >= t.n) break;      // 8 bits: a wave works on its block as a whole
+            f32x4 g = {0.f, 0.f, 0.f, 0.f}, p = g, m = g, v = g;
+            if (i < t.n) {
+                g = load4(gp, t.g_type, i, t.n);
+                p = load4(t.p, t.p_type, i, t.n);
+            }
+            float sm = 0.f, sv = 0.f;
+            const int64_t blk = (t.off + i) / kBlock;
+            if (BITS == 32) {
+                m = load4((const float *)a.m + t.off, PPO2HIP_F32, i, t.n);
+                v = load4((const float *)a.v + t.off, PPO2HIP_F32, i, t.n);
+            } else {
+                const unsigned mc = ((const unsigned *)a.m)[(t.off + i) / 4], vc = ((const unsigned *)a.v)[(t.off + i) / 4];
+                sm = a.m_scale[blk];
+                sv = a.v_scale[blk];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    m[k] = moment_of((int8_t)(mc >> (8 * k)), sm);
+                    v[k] = square_of((uint8_t)(vc >> (8 * k)), sv);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const float gs = g[k] * scale;
+                m[k] = a.b1 * m[k] + a.omb1 * gs;
+                v[k] = a.b2 * v[k] + a.omb2 * (gs * gs);
+                p[k] = p[k] - a.lr * (m[k] * a.c1 / (sqrtf(v[k] * a.c2) + a.eps) + wd * p[k]);
+            }
+            if (i < t.n) store4(t.p, t.p_type, i, t.n, p);
+            if (BITS == 32) {
+                store4((float *)a.m + t.off, PPO2HIP_F32, i, t.n, m);
+                store4((float *)a.v + t.off, PPO2HIP_F32, i, t.n, v);
+            } else {
+                // largest bit patterns: an infinity or a NaN of the block wins over every finite value, its scale becomes the
+                // block's scale and the block decodes to NaN instead of to something that looks sound
+                unsigned um = 0, uv = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (i + k >= t.n) m[k] = 0.f, v[k] = 0.f;
+                    const unsigned x = __float_as_uint(m[k]) & 0x7fffffffu, y = __float_as_uint(v[k]) & 0x7fffffffu;
+                    um = um > x ? um : x;
+                    uv = uv > y ? uv : y;
+                }
+                um = wave_umax(um);
+                uv = wave_umax(uv);
+                const bool sound_m = um < 0x7f800000u, sound_v = uv < 0x7f800000u;
+                sm = sound_m ? __uint_as_float(um) : __builtin_nanf("");
+                sv = sound_v ? __uint_as_float(uv) : __builtin_nanf("");
+                const float im = sm > 0.f ? 127.f / sqrtf(sm) : 0.f, iv = sv > 0.f ? 255.f / sqrtf(sqrtf(sv)) : 0.f;
+                unsigned mc = 0, vc = 0;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const float x = sound_m ? rintf(sqrtf(fabsf(m[k])) * im) : 0.f, y = sound_v ? rintf(sqrtf(sqrtf(v[k])) * iv) : 0.f;
+                    int cm = (int)fminf(x, 127.f), cv = (int)fminf(y, 255.f);
+                    if (cv == 0 && sound_v && v[k] > 0.f) cv = 1;
+                    cm = m[k] < 0.f ? -cm : cm;
+                    mc |= (unsigned)(cm & 255) << (8 * k);
+                    vc |= (unsigned)cv << (8 * k);
+                }
+                ((unsigned *)a.m)[(t.off + i) / 4] = mc;
+                ((unsigned *)a.v)[(t.off + i) / 4] = vc;
+                if ((threadIdx.x & 63) == 0) {
+                    a.m_scale[blk] = sm;
+                    a.v_scale[blk] = sv;
+                }
+            }
+        }
+    }
+}
+
+// moments as the values they stand for, packed in list order (no padding between tensors)
+template <class T>
+__global__ __launch_bounds__(kThreads) void adamw_state_kernel(const TensorRow *tensors, const ChunkRow *chunks, const int64_t *packed, int nchunks,
+                                                               const unsigned *mc_, const unsigned *vc_, const float *m_scale, const float *v_scale,
+                                                               T *m_out, T *v_out) {
+    for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
+        const ChunkRow ch = chunks[c];
+        const TensorRow &t = tensors[ch.tensor];
+        const int64_t at = packed[ch.tensor];
+#pragma unroll
+        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
+            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
+            if (i >= t.n) break;
+            const unsigned mc = mc_[(t.off + i) / 4], vc = vc_[(t.off + i) / 4];
+            const float sm = m_scale[(t.off + i) / kBlock], sv = v_scale[(t.off + i) / kBlock];
+            f32x4 m, v;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                m[k] = moment_of((int8_t)(mc >> (8 * k)), sm);
+                v[k] = square_of((uint8_t)(vc >> (8 * k)), sv);
+            }
+            const int type = sizeof(T) == 4 ? PPO2HIP_F32 : PPO2HIP_BF16;
+            store4(m_out + at, type, i, t.n, m);
+            store4(v_out + at, type, i, t.n, v);
+        }
+    }
+}
+
+}  // namespace ppo2hip
+
+using namespace ppo2hip;
+
+static int64_t chunks_of(int64_t n) { return ceil_div(n, kChunk); }
+
+static int adamw_check(const char *what, const ppo2hip_adamw_tensor *t, int nt, int bits) {
+    PPO2HIP_REQUIRE(nt >= 0 && (t || nt == 0), "%s: bad tensor list", what);
+    PPO2HIP_REQUIRE(bits == 32 || bits == 8, "%s: moments in %d bits (32 and 8 exist)", what, bits);
+    int64_t chunks = 0;
+    for (int k = 0; k < nt; k++) {
+        PPO2HIP_REQUIRE(t[k].n >= 0 && (t[k].param || t[k].n == 0), "%s: tensor %d is null or has a negative size", what, k);
+        PPO2HIP_REQUIRE((t[k].param_dtype == PPO2HIP_F32 || t[k].param_dtype == PPO2HIP_BF16) &&
+                            (t[k].grad_dtype == PPO2HIP_F32 || t[k].grad_dtype == PPO2HIP_BF16),
+                        "%s: tensor %d: parameters and gradients are float32 or bfloat16", what, k);
+        PPO2HIP_REQUIRE(t[k].n <= (1ll << 42), "%s: tensor %d is too large", what, k);
+        chunks += chunks_of(t[k].n);
+    }
+    PPO2HIP_REQUIRE(chunks <= 0x7fffffffll, "%s: list too large", what);
+    return PPO2HIP_OK;
+}
+
+struct PlanShape {
+    size_t chunk_off, packed_off, bytes;
+};
+static PlanShape plan_shape(const ppo2hip_adamw_tensor *t, int nt) {
+    int64_t chunks = 0;
+    for (int k = 0; k < nt; k++) chunks += chunks_of(t[k].n);
+    PlanShape s;
+    s.packed_off = align_up(nt * sizeof(TensorRow), 16);
+    s.chunk_off = align_up(s.packed_off + nt * sizeof(int64_t), 16);
+    s.bytes = align_up(s.chunk_off + chunks * sizeof(ChunkRow), 16) + 16;
+    return s;
+}
+
+extern "C" int64_t ppo2hip_adamw_state_elements(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits) {
+    int rc = adamw_check("adamw_state_elements", tensors, ntensors, state_bits);
+    if (rc) return rc;
+    int64_t n = 0;
+    for (int k = 0; k < ntensors; k++) n += state_bits == 32 ? tensors[k].n : ceil_div(tensors[k].n, kBlock) * kBlock;
+    return n;
+}
+
+extern "C" size_t ppo2hip_adamw_plan_bytes(const ppo2hip_adamw_tensor *tensors, int ntensors) {
+    if (adamw_check("adamw_plan_bytes", tensors, ntensors, 32)) return 0;
+    return plan_shape(tensors, ntensors).bytes;
+}
+
+extern "C" int ppo2hip_adamw_plan_fill(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, void *image, size_t image_bytes) {
+    int rc = adamw_check("adamw_plan_fill", tensors, ntensors, state_bits);
+    if (rc) return rc;
+    const PlanShape s = plan_shape(tensors, ntensors);
+    PPO2HIP_REQUIRE(image, "adamw_plan_fill: image is null");
+    if (image_bytes < s.bytes) {
+        set_error("adamw_plan_fill: image of %zu bytes, %zu needed", image_bytes, s.bytes);
+        return PPO2HIP_ENOSPACE;
+    }
+    TensorRow *rows = (TensorRow *)image;
+    int64_t *packed = (int64_t *)((char *)image + s.packed_off);
+    ChunkRow *chunks = (ChunkRow *)((char *)image + s.chunk_off);
+    int64_t off = 0, at = 0;
+    for (int k = 0; k < ntensors; k++) {
+        const ppo2hip_adamw_tensor &t = tensors[k];
+        rows[k] = TensorRow{t.param, t.n, off, t.param_dtype, t.grad_dtype, t.decay, 0};
+        packed[k] = at;
+        for (int64_t c = 0; c < chunks_of(t.n); c++) *chunks++ = ChunkRow{k, (int32_t)c};
+        off += state_bits == 32 ? t.n : ceil_div(t.n, kBlock) * kBlock;
+        at += t.n;
+    }
+    return PPO2HIP_OK;
+}
+
+extern "C" size_t ppo2hip_adamw_workspace_bytes(const ppo2hip_adamw_tensor *tensors, int ntensors) {
+    (void)tensors;
+    const int64_t launches = ceil_div(ntensors > 0 ? ntensors : 1, kMaxGrads);
+    return (size_t)launches * kNormGroups * sizeof(double);
+}
+
+extern "C" int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, const void *plan, const void *const *grads,
+                                  void *m, float *m_scale, void *v, float *v_scale, double lr, int64_t t, double beta1, double beta2,
+                                  double epsilon, double weight_decay, double grad_scale, double max_grad_norm, float *norm_out,
+                                  void *workspace, size_t workspace_bytes, void *stream) {
+    int rc = adamw_check("adamw_step", tensors, ntensors, state_bits);
+    if (rc) return rc;
+    PPO2HIP_REQUIRE(t >= 1, "adamw_step: step count t=%lld must be at least 1", (long long)t);
+    PPO2HIP_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw_step: beta1=%g, beta2=%g outside [0, 1)", beta1, beta2);
+    PPO2HIP_REQUIRE(epsilon >= 0.0, "adamw_step: epsilon=%g is negative", epsilon);
+    const PlanShape shape = plan_shape(tensors, ntensors);
+    int64_t total = 0;
+    for (int k = 0; k < ntensors; k++) total += tensors[k].n;
+    if (total == 0) return PPO2HIP_OK;
+    PPO2HIP_REQUIRE(plan && grads && m && v, "adamw_step: null pointer");
+    PPO2HIP_REQUIRE(state_bits == 32 || (m_scale && v_scale), "adamw_step: 8-bit moments need their scales");
+    const bool clip = max_grad_norm > 0.0;
+    if (clip && (!workspace || workspace_bytes < ppo2hip_adamw_workspace_bytes(tensors, ntensors))) {
+        set_error("adamw_step: workspace of %zu bytes, %zu needed to clip", workspace ? workspace_bytes : (size_t)0,
+                  ppo2hip_adamw_workspace_bytes(tensors, ntensors));
+        return PPO2HIP_ENOSPACE;
+    }
+    hipStream_t s = (hipStream_t)stream;
+    const TensorRow *rows = (const TensorRow *)plan;
+    const ChunkRow *chunks = (const ChunkRow *)((const char *)plan + shape.chunk_off);
+    double *partial = (double *)workspace;
+    int npartial = 0;
+    if (clip) {
+        int64_t chunk = 0;
+        for (int k0 = 0; k0 < ntensors; k0 += kMaxGrads) {
+            NormArgs a;
+            a.tensors = rows;
+            a.chunks = chunks + chunk;
+            a.first_tensor = k0;
+            a.partial = partial + npartial;
+            a.gscale = (float)grad_scale;
+            int64_t here = 0;
+            for (int k = k0; k < ntensors && k < k0 + kMaxGrads; k++) {
+                a.g[k - k0] = grads[k];
+                here += chunks_of(tensors[k].n);
+            }
+            a.nchunks = (int32_t)here;
+            chunk += here;
+            if (here == 0) continue;
+            const int groups = (int)(here < kNormGroups ? here : kNormGroups);
+            hipLaunchKernelGGL(adamw_norm_kernel, dim3(groups), dim3(kThreads), 0, s, a);
+            if ((rc = check_launch("adamw_norm_kernel"))) return rc;
+            npartial += groups;
+        }
+    }
+    AdamwArgs a;
+    a.tensors = rows;
+    a.m = m;
+    a.v = v;
+    a.m_scale = m_scale;
+    a.v_scale = v_scale;
+    a.partial = partial;
+    a.npartial = npartial;
+    a.lr = (float)lr;
+    a.c1 = (float)(1.0 / (1.0 - pow(beta1, (double)t)));
+    a.c2 = (float)(1.0 / (1.0 - pow(beta2, (double)t)));
+    a.b1 = (float)beta1;
+    a.b2 = (float)beta2;
+    a.omb1 = (float)(1.0 - beta1);               // formed in 64 bits: 1.f - 0.999f is off by 4.7e-5 of its value
+    a.omb2 = (float)(1.0 - beta2);
+    a.eps = (float)epsilon;
+    a.wd = (float)weight_decay;
+    a.gscale = (float)grad_scale;
+    a.max_norm = clip ? (float)max_grad_norm : 0.f;
+    a.norm_out = norm_out;
+    int64_t chunk = 0;
+    for (int k0 = 0; k0 < ntensors; k0 += kMaxGrads) {
+        a.first_tensor = k0;
+        a.chunks = chunks + chunk;
+        int64_t here = 0;
+        for (int k = k0; k < ntensors && k < k0 + kMaxGrads; k++) {
+            a.g[k - k0] = grads[k];
+            here += chunks_of(tensors[k].n);
+        }
+        a.nchunks = (int32_t)here;
+        chunk += here;
+        if (here == 0) continue;
+        const int64_t groups = here < 2048 ? here : 2048;
+        if (state_bits == 32)
+            hipLaunchKernelGGL(adamw_kernel<32>, dim3((unsigned)groups), dim3(kThreads), 0, s, a);
+        else
+            hipLaunchKernelGGL(adamw_kernel<8>, dim3((unsigned)groups), dim3(kThreads), 0, s, a);
+        if ((rc = check_launch("adamw_kernel"))) return rc;
+        a.norm_out = nullptr;
+    }
+    return PPO2HIP_OK;
+}
+
+extern "C" int ppo2hip_adamw_state(const ppo2hip_adamw_tensor *tensors, int ntensors, const void *plan, const void *m, const float *m_scale,
+                                   const void *v, const float *v_scale, int out_dtype, void *m_out, void *v_out, void *stream) {
+    int rc = adamw_check("adamw_state", tensors, ntensors, 8);
+    if (rc) return rc;
+    PPO2HIP_REQUIRE(out_dtype == PPO2HIP_F32 || out_dtype == PPO2HIP_BF16, "adamw_state: outputs are float32 or bfloat16");
+    int64_t nchunks = 0;
+    for (int k = 0; k < ntensors; k++) nchunks += chunks_of(tensors[k].n);
+    if (nchunks == 0) return PPO2HIP_OK;
+    PPO2HIP_REQUIRE(plan && m && m_scale && v && v_scale && m_out && v_out, "adamw_state: null pointer");
+    const PlanShape shape = plan_shape(tensors, ntensors);
+    const TensorRow *rows = (const TensorRow *)plan;
+    const int64_t *packed = (const int64_t *)((const char *)plan + shape.packed_off);
+    const ChunkRow *chunks = (const ChunkRow *)((const char *)plan + shape.chunk_off);
+    const unsigned groups = (unsigned)(nchunks < 4096 ? nchunks : 4096);
+    hipStream_t s = (hipStream_t)stream;
+    if (out_dtype == PPO2HIP_F32)
+        hipLaunchKernelGGL(adamw_state_kernel<float>, dim3(groups), dim3(kThreads), 0, s, rows, chunks, packed, (int)nchunks, (const unsigned *)m,
+                           (const unsigned *)v, m_scale, v_scale, (float *)m_out, (float *)v_out);
+    else
+        hipLaunchKernelGGL(adamw_state_kernel<__bf16>, dim3(groups), dim3(kThreads), 0, s, rows, chunks, packed, (int)nchunks, (const unsigned *)m,
+                           (const unsigned *)v, m_scale, v_scale, (__bf16 *)m_out, (__bf16 *)v_out);
+    return check_launch("adamw_state_kernel");
+}

@@ -121,6 +121,226 @@ def sf01(arr):
 
 
 # --------------------------------------------------------------------------------------
+# gated linear recurrence
+# --------------------------------------------------------------------------------------
+
+_GLR_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _glr_seq(t, name, shape, dtype):
+    """[T, E, H] tensor with a contiguous innermost dimension and any strides over T and E."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError("%s must be a %s tensor" % (name, dtype))
+    if t.shape != shape:
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    st, se, sj = t.stride()
+    if sj != 1 and shape[2] > 1:
+        raise ValueError("%s must be contiguous over its last dimension" % name)
+    return _lib.Seq(t.data_ptr(), st, se)
+
+
+def _glr_resets(resets, shape):
+    """[T, E] flags, any strides."""
+    if resets is None:
+        return None
+    if not isinstance(resets, torch.Tensor) or resets.dtype not in (torch.bool, torch.uint8):
+        raise TypeError("resets must be a bool or uint8 tensor")
+    if resets.shape != shape[:2]:
+        raise ValueError("resets must have shape %s, got %s" % (tuple(shape[:2]), tuple(resets.shape)))
+    return _lib.Seq(resets.data_ptr(), *resets.stride())
+
+
+def _glr_f32(t, name, shape):
+    if t is None:
+        return None
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32:
+        raise TypeError("%s must be a float32 tensor" % name)
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError("%s must be contiguous with shape %s" % (name, tuple(shape)))
+    return ctypes.c_void_p(t.data_ptr())
+
+
+def _extent(t):
+    """Byte range [first, last) that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _glr_apart(out, name, others):
+    """Refuses an output tensor that a caller brings whose elements meet each other or those of another tensor.  Two tensors
+    of equal strides in one buffer are told apart when their rows take turns (the halves of a joint projection)."""
+    need = 1
+    for st, n in sorted((s, n) for n, s in zip(out.shape, out.stride()) if n > 1):
+        if st < need:
+            raise ValueError("%s overlaps itself" % name)
+        need = st * (n - 1) + need
+    a0, a1 = _extent(out)
+    for oname, o in others:
+        if o is None or o is out and oname == name:
+            continue
+        b0, b1 = _extent(o)
+        if a1 <= b0 or b1 <= a0:
+            continue
+        if o.dim() == 3 and out.dim() == 3 and o.dtype == out.dtype:
+            strides = [sorted(s for s, n in zip(t.stride()[:2], t.shape[:2]) if n > 1) for t in (o, out)]
+            H, d = out.shape[2], a0 - b0
+            if strides[0] == strides[1] and d % out.element_size() == 0:
+                d //= out.element_size()
+                if not strides[0]:
+                    if abs(d) >= H:
+                        continue
+                elif all(s % strides[0][0] == 0 for s in strides[0]) and H <= d % strides[0][0] <= strides[0][0] - H:
+                    continue
+        raise ValueError("%s overlaps %s" % (name, oname))
+
+
+def _same_gpu(first, name, tensors):
+    """Every tensor on the GPU of the first; True where that is not the current one."""
+    dev = first.device
+    if dev.type != "cuda":
+        raise TypeError("%s must be a device tensor" % name)
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise TypeError("all tensors must be on %s" % dev)
+    return dev.index != torch.cuda.current_device()
+
+
+class GlrSaved:
+    """What :func:`glr_forward` keeps for :func:`glr_backward`: the float32 states in front of every 16th step."""
+    __slots__ = ("states", "shape", "dtype")
+
+    def __init__(self, states, shape, dtype):
+        self.states, self.shape, self.dtype = states, shape, dtype
+
+
+def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want_saved=False):
+    """Gated linear recurrence over time-major sequences:
+
+        a = sigmoid(f + bias)     h[t] = a[t] * (0 where resets[t], else h[t-1]) + (1 - a[t]) * x[t]     y[t] = h[t]
+
+    ``f``, ``x`` [T, E, H] float32 / bfloat16 / float16, contiguous over H with any strides over T and E (halves of a joint
+    projection, batch-first tensors); ``resets`` [T, E] flags set BEFORE step t, as the rollout's dones are; ``bias`` [H]
+    and ``h0`` [E, H] float32 (default zeros).  Returns (y, h_last, saved): y in x's type, the last state [E, H] in float32 and,
+    with ``want_saved``, what :func:`glr_backward` needs.  ``y`` and ``h_last`` may be brought; they must not overlap each
+    other or the inputs."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _GLR_TYPES:
+        raise TypeError("x must be a float32, bfloat16 or float16 tensor [T, E, H]")
+    shape, dt = x.shape, x.dtype
+    sf, sx, sr = _glr_seq(f, "f", shape, dt), _glr_seq(x, "x", shape, dt), _glr_resets(resets, shape)
+    pb, p0 = _glr_f32(bias, "bias", shape[2:]), _glr_f32(h0, "h0", shape[1:])
+    if y is not None:
+        _glr_seq(y, "y", shape, dt)
+        _glr_apart(y, "y", (("f", f), ("x", x), ("resets", resets), ("h0", h0), ("bias", bias)))
+    if h_last is not None:
+        _glr_f32(h_last, "h_last", shape[1:])
+        _glr_apart(h_last, "h_last", (("f", f), ("x", x), ("resets", resets), ("h0", h0), ("bias", bias), ("y", y)))
+    if _same_gpu(x, "x", (f, bias, resets, h0, y, h_last)):
+        with torch.cuda.device(x.device):
+            return glr_forward(f, x, h0, resets, bias, y, h_last, want_saved)
+    T, E, H = shape
+    if y is None:
+        y = torch.empty(shape, dtype=dt, device=x.device)
+    if h_last is None:
+        h_last = torch.empty((E, H), dtype=torch.float32, device=x.device)
+    saved = None
+    if want_saved:
+        saved = GlrSaved(torch.empty((-(-T // _lib.GLR_SPAN), E, H), dtype=torch.float32, device=x.device), shape, dt)
+    _glr_call_forward(_GLR_TYPES[dt], T, E, H, sf, sx, pb, sr, p0, _lib.Seq(y.data_ptr(), *y.stride()[:2]), h_last,
+                      saved.states if saved else None, "glr_forward")
+    return y, h_last, saved
+
+
+def _glr_call_forward(code, T, E, H, f, x, bias, resets, h0, y, h_last, saved, what):
+    need = lib.ppo2hip_glr_forward_workspace_bytes(code, T, E, H)
+    ws = torch.empty(need, dtype=torch.uint8, device=h_last.device) if need else None
+    check(lib.ppo2hip_glr_forward(code, T, E, H, f, x, bias, resets, h0, y, h_last.data_ptr(), _ptr(saved), _ptr(ws), need, _stream()),
+          what)
+
+
+def glr_step(f, x, state, resets=None, bias=None, y=None):
+    """One acting step of :func:`glr_forward` for E envs: ``f``, ``x`` [E, H], ``resets`` [E]; ``state`` [E, H] float32 is advanced
+    in place.  Returns y [E, H] in x's type."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _GLR_TYPES:
+        raise TypeError("x must be a float32, bfloat16 or float16 tensor [E, H]")
+    if not isinstance(f, torch.Tensor) or f.dim() != 2:
+        raise TypeError("f must be a tensor [E, H]")
+    E, H = x.shape
+    shape, dt = (1, E, H), x.dtype
+    seqs = []
+    for t, name in ((f, "f"), (x, "x")) if y is None else ((f, "f"), (x, "x"), (y, "y")):
+        if not isinstance(t, torch.Tensor) or t.dtype != dt:
+            raise TypeError("%s must be a %s tensor" % (name, dt))
+        if t.shape != x.shape:
+            raise ValueError("%s must have shape %s, got %s" % (name, tuple(x.shape), tuple(t.shape)))
+        se, sj = t.stride()
+        if sj != 1 and H > 1:
+            raise ValueError("%s must be contiguous over its last dimension" % name)
+        seqs.append(_lib.Seq(t.data_ptr(), 0, se))
+    if state is None:
+        raise TypeError("state must be a float32 tensor")
+    pb, ps, sr = _glr_f32(bias, "bias", (H,)), _glr_f32(state, "state", (E, H)), None
+    if resets is not None:
+        if not isinstance(resets, torch.Tensor) or resets.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("resets must be a bool or uint8 tensor")
+        if resets.shape != (E,):
+            raise ValueError("resets must have shape %s, got %s" % ((E,), tuple(resets.shape)))
+        sr = _lib.Seq(resets.data_ptr(), 0, resets.stride(0))
+    if y is not None:
+        _glr_apart(y.unsqueeze(0), "y", (("f", f.unsqueeze(0)), ("x", x.unsqueeze(0)), ("state", state), ("resets", resets), ("bias", bias)))
+    if _same_gpu(x, "x", (f, bias, resets, state, y)):
+        with torch.cuda.device(x.device):
+            return glr_step(f, x, state, resets, bias, y)
+    if y is None:
+        y = torch.empty((E, H), dtype=dt, device=x.device)
+        seqs.append(_lib.Seq(y.data_ptr(), 0, H))
+    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, seqs[0], seqs[1], pb, sr, ps, seqs[2], ps, None, None, 0, _stream()), "glr_step")
+    return y
+
+
+def glr_backward(f, x, dy, saved, resets=None, bias=None, dh_last=None, df=None, dx=None):
+    """Gradients of :func:`glr_forward` from ``dy`` [T, E, H] (x's type) and ``dh_last`` [E, H] (float32, default zeros); ``f``, ``x``,
+    ``resets``, ``bias`` as the forward call had them and ``saved`` as it returned it.  Returns (df, dx, dh0, dbias): df and dx
+    in x's type (into ``df`` / ``dx`` where brought, e.g. the halves of one buffer), dh0 [E, H] and dbias [H] float32 (None
+    without ``bias``), dbias summed in a fixed order."""
+    if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _GLR_TYPES:
+        raise TypeError("x must be a float32, bfloat16 or float16 tensor [T, E, H]")
+    shape, dt = x.shape, x.dtype
+    if not isinstance(saved, GlrSaved):
+        raise TypeError("saved must be what glr_forward returned with want_saved=True")
+    if saved.shape != shape or saved.dtype != dt:
+        raise ValueError("saved belongs to a forward call on %s %s" % (tuple(saved.shape), saved.dtype))
+    sf, sx, sdy, sr = _glr_seq(f, "f", shape, dt), _glr_seq(x, "x", shape, dt), _glr_seq(dy, "dy", shape, dt), _glr_resets(resets, shape)
+    pb, pl = _glr_f32(bias, "bias", shape[2:]), _glr_f32(dh_last, "dh_last", shape[1:])
+    ins = (("f", f), ("x", x), ("dy", dy), ("resets", resets), ("bias", bias), ("dh_last", dh_last), ("saved", saved.states))
+    if df is not None:
+        _glr_seq(df, "df", shape, dt)
+        _glr_apart(df, "df", ins)
+    if dx is not None:
+        _glr_seq(dx, "dx", shape, dt)
+        _glr_apart(dx, "dx", ins + (("df", df),))
+    if _same_gpu(x, "x", (f, dy, saved.states, bias, resets, dh_last, df, dx)):
+        with torch.cuda.device(x.device):
+            return glr_backward(f, x, dy, saved, resets, bias, dh_last, df, dx)
+    T, E, H = shape
+    dev = x.device
+    if df is None:
+        df = torch.empty(shape, dtype=dt, device=dev)
+    if dx is None:
+        dx = torch.empty(shape, dtype=dt, device=dev)
+    dh0 = torch.empty((E, H), dtype=torch.float32, device=dev)
+    dbias = None if bias is None else torch.empty(H, dtype=torch.float32, device=dev)
+    code = _GLR_TYPES[dt]
+    need = lib.ppo2hip_glr_backward_workspace_bytes(code, T, E, H, int(bias is not None))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    check(lib.ppo2hip_glr_backward(code, T, E, H, sf, sx, pb, sr, saved.states.data_ptr(), sdy, pl, _lib.Seq(df.data_ptr(), *df.stride()[:2]),
+                                   _lib.Seq(dx.data_ptr(), *dx.stride()[:2]), _ptr(dbias), dh0.data_ptr(), _ptr(ws), need, _stream()),
+          "glr_backward")
+    return df, dx, dh0, dbias
+
+
+# --------------------------------------------------------------------------------------
 # env-wrapper filters
 # --------------------------------------------------------------------------------------
 
@@ -735,6 +955,137 @@ def adam_step(params, grads, m, v, lr, t, scratch, max_grad_norm=0.0, grad_scale
     check(lib.ppo2hip_adam_step(_ptr(params), _ptr(grads), _ptr(m), _ptr(v), P, float(lr), int(t), beta1, beta2,
                                 epsilon, float(grad_scale), float(max_grad_norm or 0.0), _ptr(scratch), _stream()),
           "adam_step")
+
+
+# --------------------------------------------------------------------------------------
+# AdamW over many tensors
+# --------------------------------------------------------------------------------------
+
+_ADAMW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
+
+
+class AdamWPlan:
+    """A list of parameter tensors with their AdamW moments, laid out once for :func:`adamw_step`.
+
+    ``params``: contiguous float32 / bfloat16 device tensors of one GPU that do not overlap (views into one arena are
+    fine); they are updated in place.  ``decay``: per tensor the factor of the step's ``weight_decay`` (bools do), default 1.
+    ``grad_dtype``: type of all gradients, default each parameter's own.  ``state_bits`` 32 keeps the moments as two packed
+    float32 arrays in list order (``plan.m``, ``plan.v``), 8 as codes with one float32 scale per block of 256 elements of a
+    tensor (``plan.m`` int8, ``plan.v`` uint8, ``plan.m_scale``, ``plan.v_scale``): 2 bytes per parameter instead of 8.
+    ``state`` adopts existing arrays, (m, v) or (m, m_scale, v, v_scale); without it the moments start at zero.
+    ``plan.norm`` is a device float32 [2]: the gradient norm (when clipping) and the factor applied to the gradients."""
+
+    def __init__(self, params, state_bits=32, decay=None, state=None, grad_dtype=None):
+        params = list(params)
+        if not params:
+            raise ValueError("AdamWPlan needs at least one tensor")
+        if state_bits not in (32, 8):
+            raise ValueError("state_bits must be 32 or 8")
+        if grad_dtype is not None and grad_dtype not in _ADAMW_TYPES:
+            raise TypeError("grad_dtype must be float32 or bfloat16")
+        for k, p in enumerate(params):
+            if not isinstance(p, torch.Tensor) or p.dtype not in _ADAMW_TYPES:
+                raise TypeError("params[%d] must be a float32 or bfloat16 tensor" % k)
+            if not p.is_contiguous():
+                raise ValueError("params[%d] must be contiguous" % k)
+        decay = [1.0] * len(params) if decay is None else [float(d) for d in decay]
+        if len(decay) != len(params):
+            raise ValueError("decay must have one entry per tensor")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in params if p.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("params overlap (is one of them listed twice?)")
+        dev = params[0].device
+        for k, p in enumerate(params):
+            if not p.is_cuda or p.device != dev:
+                raise TypeError("params[%d] must be a tensor of the first one's GPU" % k)
+        self.device, self.state_bits = dev, state_bits
+        self.params = [p.detach() for p in params]
+        self.grad_dtypes = [grad_dtype or p.dtype for p in params]
+        self._ptrs = [p.data_ptr() for p in params]
+        self._numels = [p.numel() for p in params]
+        n = len(params)
+        self._tensors = (_lib.AdamwTensor * n)(*[
+            _lib.AdamwTensor(p.data_ptr() if p.numel() else None, p.numel(), _ADAMW_TYPES[p.dtype], _ADAMW_TYPES[g], d, 0)
+            for p, g, d in zip(params, self.grad_dtypes, decay)])
+        elems = int(lib.ppo2hip_adamw_state_elements(self._tensors, n, state_bits))
+        if elems < 0:
+            check(elems, "adamw_state_elements")
+        self.numel = sum(self._numels)
+        blocks = elems // _lib.ADAMW_BLOCK
+        with torch.cuda.device(dev):
+            if state is None:
+                zeros = lambda count, dt: torch.zeros(count, dtype=dt, device=dev)      # noqa: E731
+                state = ((zeros(elems, torch.float32), zeros(elems, torch.float32)) if state_bits == 32 else
+                         (zeros(elems, torch.int8), zeros(blocks, torch.float32), zeros(elems, torch.uint8), zeros(blocks, torch.float32)))
+            want = ([("m", torch.float32, elems), ("v", torch.float32, elems)] if state_bits == 32 else
+                    [("m", torch.int8, elems), ("m_scale", torch.float32, blocks), ("v", torch.uint8, elems), ("v_scale", torch.float32, blocks)])
+            if len(state) != len(want):
+                raise ValueError("state must hold %s" % ", ".join(w[0] for w in want))
+            self.m_scale = self.v_scale = None
+            for t, (name, dt, count) in zip(state, want):
+                if _dev(t, dt, name).numel() != count or t.device != dev:
+                    raise ValueError("state %s must hold %d entries on %s" % (name, count, dev))
+                if state_bits == 8 and t.data_ptr() % 4:
+                    raise ValueError("state %s must be aligned to 4 bytes" % name)
+                setattr(self, name, t)
+            image = np.zeros(int(lib.ppo2hip_adamw_plan_bytes(self._tensors, n)), np.uint8)
+            check(lib.ppo2hip_adamw_plan_fill(self._tensors, n, state_bits, image.ctypes.data_as(ctypes.c_void_p), image.size),
+                  "adamw_plan_fill")
+            self._image = torch.from_numpy(image).to(dev)
+            self._ws_bytes = int(lib.ppo2hip_adamw_workspace_bytes(self._tensors, n))
+            self._ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev)
+            self.norm = torch.zeros(2, dtype=torch.float32, device=dev)
+        self._grads = (ctypes.c_void_p * n)()
+        self._fixed = tuple(_ptr(t) for t in (self._image, self.m, self.m_scale, self.v, self.v_scale, self.norm, self._ws))
+
+    def _grad_ptrs(self, grads):
+        if len(grads) != len(self._ptrs):
+            raise ValueError("adamw_step needs one gradient (or None) per tensor: %d for %d" % (len(grads), len(self._ptrs)))
+        ptrs, dev = self._grads, self.device
+        for k, g in enumerate(grads):
+            if g is None:
+                ptrs[k] = None
+                continue
+            if g.dtype != self.grad_dtypes[k] or g.device != dev:
+                raise TypeError("grads[%d] must be %s on %s" % (k, self.grad_dtypes[k], dev))
+            if g.numel() != self._numels[k] or not g.is_contiguous():
+                raise ValueError("grads[%d] must be contiguous with %d entries" % (k, self._numels[k]))
+            ptrs[k] = g.data_ptr() or None
+        for k, p in enumerate(self.params):
+            if p.data_ptr() != self._ptrs[k]:
+                raise ValueError("params[%d] has moved since the plan was made" % k)
+        return ptrs
+
+
+def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, max_grad_norm=0.0, grad_scale=1.0):
+    """One AdamW step of every tensor of ``plan``: step count ``t`` (1 for the first), gradients in list order (contiguous; None
+    leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by the norm over all of them when
+    ``max_grad_norm`` > 0.  Bias-corrected roots next to ``epsilon`` and decay apart from the gradient: unlike :func:`adam_step`,
+    which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  A HIP graph that captures the call keeps ``lr`` and ``t``."""
+    if plan.device.index != torch.cuda.current_device():
+        with torch.cuda.device(plan.device):
+            return adamw_step(plan, grads, lr, t, beta1, beta2, epsilon, weight_decay, max_grad_norm, grad_scale)
+    ptrs = plan._grad_ptrs(grads)
+    image, m, ms, v, vs, norm, ws = plan._fixed
+    check(lib.ppo2hip_adamw_step(plan._tensors, len(ptrs), plan.state_bits, image, ptrs, m, ms, v, vs, lr, t, beta1, beta2, epsilon,
+                                 weight_decay, grad_scale, max_grad_norm or 0.0, norm, ws, plan._ws_bytes, _stream()), "adamw_step")
+
+
+def adamw_state(plan, dtype=torch.float32):
+    """The moments of ``plan`` as values: two packed tensors [numel] in list order.  For 32-bit moments the plan's own arrays
+    (dtype float32); for 8-bit ones new arrays of ``dtype`` (float32 or bfloat16)."""
+    if dtype not in _ADAMW_TYPES or (plan.state_bits == 32 and dtype != torch.float32):
+        raise TypeError("dtype must be float32, or bfloat16 for 8-bit moments")
+    if plan.state_bits == 32:
+        return plan.m, plan.v
+    if plan.device.index != torch.cuda.current_device():
+        with torch.cuda.device(plan.device):
+            return adamw_state(plan, dtype)
+    m, v = (torch.empty(plan.numel, dtype=dtype, device=plan.device) for _ in range(2))
+    image, mp, ms, vp, vs, _, _ = plan._fixed
+    check(lib.ppo2hip_adamw_state(plan._tensors, len(plan._ptrs), image, mp, ms, vp, vs, _ADAMW_TYPES[dtype], _ptr(m), _ptr(v),
+                                  _stream()), "adamw_state")
+    return m, v
 
 
 class NativeComm:

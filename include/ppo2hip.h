@@ -471,6 +471,95 @@ int ppo2hip_ppo_epoch_shares(const ppo2hip_policy_desc *desc, const ppo2hip_loss
                              double max_grad_norm, float *losses, void *workspace, size_t workspace_bytes,
                              void *adam_scratch, ppo2hip_comm *comm, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Gated linear recurrence
+ * ---------------------------------------------------------------------- */
+
+/* A recurrent layer whose recurrence is linear in its state, so that a sequence is a scan over time.  It has no counterpart
+ * in the reference; its masks are those of the reference's LSTM (a flag set BEFORE step t empties the state,
+ * baselines/a2c/utils.py:86-147).  Per env e and channel j:
+ *   a[t] = sigmoid(f[t] + bias)     p[t] = resets[t] ? 0 : h[t-1]     h[t] = a[t] p[t] + (1 - a[t]) x[t]     y[t] = h[t]
+ * A state that a reset empties has no influence on what follows, infinities and NaN included.  The state, both scans, the
+ * sums and everything between loads and stores are float32. */
+enum { PPO2HIP_F32 = 0, PPO2HIP_BF16 = 1, PPO2HIP_F16 = 2 };
+#define PPO2HIP_GLR_SPAN 16    /* steps between two kept states */
+
+/* A time-major [T, E, H] array with strides of its own, in elements: (t, e, j) stands at data[t*t_stride + e*e_stride + j].
+ * Halves of one projection, batch-first tensors and broadcast inputs (stride 0) are all read in place; what is written
+ * must not overlap itself or any input. */
+typedef struct ppo2hip_seq {
+    void *data;
+    int64_t t, e;
+} ppo2hip_seq;
+
+/* Forward over T steps (T = 1: the acting step).
+ *   dtype : PPO2HIP_* type of f, x and y       bias : float32 [H] or NULL       resets : uint8 flags [T, E] with strides, or NULL
+ *   h0 : float32 [E, H] or NULL (zeros)        h_last : float32 [E, H] out or NULL; may be h0 itself when T = 1
+ *   saved : float32 [ppo2hip_glr_saved_floats(T, E, H)] out or NULL: the states in front of steps 0, SPAN, 2 SPAN, ...,
+ *           which ppo2hip_glr_backward recomputes the others from
+ *   workspace : ppo2hip_glr_forward_workspace_bytes(...) bytes (may be 0)
+ * E*H may reach 2^31 - 1.  T = 0 copies h0 to h_last. */
+int64_t ppo2hip_glr_saved_floats(int T, int E, int H);
+size_t ppo2hip_glr_forward_workspace_bytes(int dtype, int T, int E, int H);
+int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias,
+                        const ppo2hip_seq *resets, const float *h0, const ppo2hip_seq *y, float *h_last, float *saved,
+                        void *workspace, size_t workspace_bytes, void *stream);
+
+/* Gradients of the same layer from dy and dh_last (float32 [E, H] or NULL: zeros); f, x, bias, resets and saved as the
+ * forward call had and left them.
+ *   df, dx : dtype [T, E, H] out      dbias : float32 [H] out or NULL, summed over t and e in a fixed order
+ *   dh0 : float32 [E, H] out or NULL, not dh_last */
+size_t ppo2hip_glr_backward_workspace_bytes(int dtype, int T, int E, int H, int want_dbias);
+int ppo2hip_glr_backward(int dtype, int T, int E, int H, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias,
+                         const ppo2hip_seq *resets, const float *saved, const ppo2hip_seq *dy, const float *dh_last,
+                         const ppo2hip_seq *df, const ppo2hip_seq *dx, float *dbias, float *dh0, void *workspace,
+                         size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * AdamW over many tensors
+ * ---------------------------------------------------------------------- */
+
+/* One step of Adam with decoupled weight decay over a list of tensors, in one launch (two when clipping); a list of more
+ * than 448 tensors takes as many again per further 448.  Beside ppo2hip_adam_step (one flat float32 arena, epsilon next to the uncorrected root, no decay) it has
+ *   g = grad * grad_scale, times max_grad_norm / max(norm, max_grad_norm) over ALL tensors' norm when max_grad_norm > 0
+ *   m = beta1 m + (1 - beta1) g     v = beta2 v + (1 - beta2) g^2
+ *   p -= lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon) + weight_decay * decay * p)
+ * Moments in 32 bits are two packed float32 arrays in list order.  Moments in 8 bits hold, for every block of
+ * PPO2HIP_ADAMW_BLOCK elements (beginning anew with every tensor), a float32 scale and codes:
+ *   m = m_scale * sign(c) * (c/127)^2, c int8      v = v_scale * (c/255)^4, c uint8, never 0 where v > 0
+ * with the scales the block's largest |m| and v, codes rounded to nearest; the step itself uses the moments before that rounding.
+ * A block that held an infinity or a NaN has NaN for its scale.  Gradients of tensors that had none are NULL: the tensor,
+ * its moments and the norm then go without it. */
+#define PPO2HIP_ADAMW_BLOCK 256
+typedef struct ppo2hip_adamw_tensor {
+    void *param;            /* DEVICE, n elements; tensors of one list must not overlap */
+    int64_t n;
+    int32_t param_dtype;    /* PPO2HIP_F32 or PPO2HIP_BF16 */
+    int32_t grad_dtype;
+    float decay;            /* factor of weight_decay for this tensor */
+    int32_t reserved;
+} ppo2hip_adamw_tensor;
+
+/* elements of each moment array (8 bits: whole blocks per tensor, the scales are this / PPO2HIP_ADAMW_BLOCK), or < 0 */
+int64_t ppo2hip_adamw_state_elements(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits);
+/* The list's device image, laid out once: fill a HOST buffer of plan_bytes, copy it to the device, hand that to the calls. */
+size_t ppo2hip_adamw_plan_bytes(const ppo2hip_adamw_tensor *tensors, int ntensors);
+int ppo2hip_adamw_plan_fill(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, void *image, size_t image_bytes);
+size_t ppo2hip_adamw_workspace_bytes(const ppo2hip_adamw_tensor *tensors, int ntensors);
+/*   tensors : HOST, as the plan was filled from     plan : DEVICE image     grads : HOST array of DEVICE pointers or NULLs
+ *   m, v : DEVICE moments (float32, or int8 / uint8 codes)     m_scale, v_scale : DEVICE float32, 8 bits only
+ *   norm_out : DEVICE float[2] or NULL: {norm of grad * grad_scale (written when clipping), factor applied to grads}
+ *   workspace : DEVICE, ppo2hip_adamw_workspace_bytes bytes, only used when clipping
+ * All host arguments are read before the call returns; a HIP graph that captures the call keeps their values. */
+int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, const void *plan,
+                       const void *const *grads, void *m, float *m_scale, void *v, float *v_scale, double lr, int64_t t,
+                       double beta1, double beta2, double epsilon, double weight_decay, double grad_scale,
+                       double max_grad_norm, float *norm_out, void *workspace, size_t workspace_bytes, void *stream);
+/* 8-bit moments as the values they stand for: packed arrays in list order, float32 or bfloat16 (out_dtype). */
+int ppo2hip_adamw_state(const ppo2hip_adamw_tensor *tensors, int ntensors, const void *plan, const void *m,
+                        const float *m_scale, const void *v, const float *v_scale, int out_dtype, void *m_out, void *v_out,
+                        void *stream);
+
 /* out[c] = scale * sum_r rows[r*stride + c] for c < ncols (<= 16): the mean of the per-minibatch
  * loss rows that learn reports, baselines/ppo2/ppo2.py:139 (scale = 1/nrows; data-parallel runs
  * fold 1/size in and SUM-all-reduce the result).  float64 sums, fixed order. */

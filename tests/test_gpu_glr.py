@@ -1,0 +1,389 @@
+"""The gated linear recurrence on the GPU against its definition in 64 bits: sizes, types, layouts, masks, edges, streams and
+graphs.  Tolerances are the worst cases derived in tests/glr_reference.py plus half a step of the output's type."""
+import pytest
+import torch
+
+from tests import glr_reference as ref
+
+pytestmark = pytest.mark.gpu
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def hip():
+    from baselines_amd import hip
+    return hip
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def layout(kind, T, E, H, dtype, fill):
+    """[T, E, H] tensor of the given layout with values from `fill`, and the buffer that it lives in."""
+    if kind == "joint":
+        buf = torch.empty((T, E, 2 * H), dtype=dtype, device="cuda")
+        t = buf[..., H:]
+    elif kind == "batch first":
+        buf = torch.empty((E, T, H), dtype=dtype, device="cuda")
+        t = buf.transpose(0, 1)
+    elif kind == "odd":                     # rows at odd addresses, gaps between rows and steps
+        buf = torch.empty(3 + T * (E * (H + 3) + 5), dtype=dtype, device="cuda")
+        t = buf[3:].as_strided((T, E, H), (E * (H + 3) + 5, H + 3, 1), 3)
+    else:
+        buf = t = torch.empty((T, E, H), dtype=dtype, device="cuda")
+    if fill is not None:
+        t.copy_(fill)
+    return t, buf
+
+
+def make(T, E, H, dtype, kind="apart", resets=False, bias=False, h0=True, seed=0, reach=6.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    normal = lambda *s: torch.randn(s, generator=g, device="cuda")      # noqa: E731
+    f = layout(kind, T, E, H, dtype, normal(T, E, H) + (0 if bias else 1) * reach * torch.rand(H, generator=g, device="cuda"))[0]
+    x = layout(kind, T, E, H, dtype, normal(T, E, H))[0]
+    return dict(f=f, x=x, h0=normal(E, H) if h0 else None,
+                resets=(torch.rand((T, E), generator=g, device="cuda") < 0.1) if resets else None,
+                bias=reach * torch.rand(H, generator=g, device="cuda") if bias else None), normal
+
+
+def close(got, want, tol, what):
+    """|got - want| <= tol + half a step of got's type at the value."""
+    assert got.shape == want.shape, what
+    err = (got.double() - want).abs()
+    bound = tol + (half_step(got.dtype) * want.abs() if got.dtype != torch.float32 else 0.0)
+    if got.dtype == F16:
+        bound = bound + 2.0 ** -25          # half a step of the smallest float16 numbers
+    if got.dtype != torch.float32:
+        bound = bound * (1 + 2 * half_step(got.dtype))
+    bad = ~(err <= bound)
+    assert not bool(bad.any()), (what, float(err[bad].max()), "of bound", float((err / bound.clamp(min=1e-300)).max()), int(bad.sum()))
+
+
+def check(hip, a, normal, dtype, kind="apart", dh_last=True, backward=True):
+    T, E, H = a["x"].shape
+    y, h_last, saved = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    want, last, _ = ref.forward(a["f"], a["x"], a["h0"], a["resets"], a["bias"])
+    b = ref.Bounds(a["f"], a["x"], a["h0"], a["resets"], a["bias"])
+    assert y.dtype == dtype and h_last.dtype == F32
+    close(y, want, b.h, "y")
+    close(h_last, last, b.h, "h_last")
+    if not backward:
+        return
+    dy = layout(kind, T, E, H, dtype, normal(T, E, H))[0]
+    dl = normal(E, H) if dh_last else None
+    df, dx, dh0, dbias = hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"], dh_last=dl)
+    wf, wx, w0, wb = ref.backward(a["f"], a["x"], a["h0"], a["resets"], a["bias"], dy, dl)
+    tg, tx, tf = b.grads(ref.largest_g(a["f"], a["bias"], a["resets"], dy, dl))
+    close(df, wf, tf, "df")
+    close(dx, wx, tx, "dx")
+    close(dh0, w0, tg, "dh0")
+    if a["bias"] is None:
+        assert dbias is None
+    else:
+        # every term's own error, and float32 sums of at most 64 terms in a row (64 U of the terms' sizes) before they widen
+        close(dbias, wb, T * tf.sum(0) + 64 * ref.U * wf.abs().sum((0, 1)) + ref.U * wb.abs(), "dbias")
+
+
+SIZES = [(1, 1, 1), (1, 37, 333), (2, 3, 5), (15, 2, 64), (16, 1, 128), (17, 4, 65), (31, 1, 200), (33, 5, 7), (64, 1, 1), (100, 3, 130),
+         (255, 2, 96), (256, 1, 64), (257, 2, 64), (513, 2, 70), (1001, 7, 33), (2049, 1, 258), (5000, 1, 64), (3, 300, 256), (128, 64, 256),
+         (40, 1, 2048), (777, 1, 1000)]
+
+
+@pytest.mark.parametrize("T,E,H", SIZES)
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_sizes(hip, T, E, H, dtype):
+    k = T + E + H
+    a, normal = make(T, E, H, dtype, resets=k % 2 == 0, bias=k % 3 != 0, h0=k % 5 != 0, seed=k)
+    check(hip, a, normal, dtype)
+
+
+@pytest.mark.parametrize("kind", ["joint", "batch first", "odd"])
+@pytest.mark.parametrize("T,E,H", [(70, 3, 64), (300, 2, 129), (19, 33, 256), (1, 5, 130)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layouts(hip, kind, T, E, H, dtype):
+    a, normal = make(T, E, H, dtype, kind=kind, resets=True, bias=True, seed=T)
+    if kind == "batch first":
+        a["resets"] = a["resets"].t().contiguous().t()
+    check(hip, a, normal, dtype, kind)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("T,E,H", [(300, 2, 129), (20, 3, 64)])
+def test_outputs_into_views_leave_the_rest_alone(hip, dtype, T, E, H):
+    a, normal = make(T, E, H, dtype, resets=True, bias=True)
+    y, ybuf = layout("odd", T, E, H, dtype, None)
+    ybuf.fill_(7.0)
+    keep = torch.ones_like(ybuf, dtype=torch.bool)
+    keep[3:].as_strided(y.shape, y.stride(), 3).fill_(False)
+    hbuf = torch.full((E + 2, H), 7.0, device="cuda")
+    want, last, saved = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    got = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], y=y, h_last=hbuf[1:E + 1])
+    assert got[0] is y and got[2] is None
+    assert torch.equal(y, want) and torch.equal(hbuf[1:E + 1], last)
+    assert bool((ybuf[keep] == 7.0).all()) and bool((hbuf[0] == 7).all()) and bool((hbuf[E + 1] == 7).all())
+    dy = normal(T, E, H).to(dtype)
+    wf, wx, w0, wb = hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"])
+    joint = torch.full((T + 1, E, 2 * H), 7.0, dtype=dtype, device="cuda")
+    df, dx, d0, db = hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"], df=joint[:T, :, :H], dx=joint[:T, :, H:])
+    assert torch.equal(joint[:T, :, :H], wf) and torch.equal(joint[:T, :, H:], wx) and bool((joint[T] == 7).all())
+    assert torch.equal(d0, w0) and torch.equal(db, wb)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_broadcast_inputs(hip, dtype):
+    T, E, H = 50, 6, 96
+    a, normal = make(T, E, H, dtype, bias=True)
+    a["f"] = a["f"][:, :1].expand(T, E, H)          # one gate for all envs
+    a["x"] = a["x"][:1].expand(T, E, H)             # one input for all steps
+    a["resets"] = (torch.rand(T, 1, device="cuda") < 0.1).expand(T, E)
+    check(hip, a, normal, dtype)
+
+
+@pytest.mark.parametrize("T", [1, 40, 700])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_masks_that_leave_nothing(hip, T, dtype):
+    a, normal = make(T, 3, 70, dtype, bias=True)
+    a["resets"] = torch.zeros(T, 3, dtype=torch.bool, device="cuda")
+    a["resets"][:, 0] = True                        # a state that never survives
+    a["resets"][0, 1] = True
+    check(hip, a, normal, dtype)
+
+
+@pytest.mark.parametrize("T", [5, 40, 700])
+def test_what_a_reset_hides_has_no_influence(hip, T):
+    """A first state and inputs that are not numbers, in front of a reset: nothing of them behind it, in either direction."""
+    E, H, r = 2, 70, T // 2
+    a, normal = make(T, E, H, F32, bias=True)
+    a["resets"] = torch.zeros(T, E, dtype=torch.uint8, device="cuda")
+    a["resets"][r] = 3                              # any value but zero is a flag
+    dy = normal(T, E, H)
+    clean = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    gclean = hip.glr_backward(a["f"], a["x"], dy, clean[2], resets=a["resets"], bias=a["bias"])
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        h0, x = a["h0"].clone(), a["x"].clone()
+        h0[0, 3] = bad
+        x[r - 1, 1, 5] = bad
+        y, last, saved = hip.glr_forward(a["f"], x, h0, resets=a["resets"], bias=a["bias"], want_saved=True)
+        assert torch.equal(y[r:], clean[0][r:]) and torch.equal(last, clean[1])
+        assert not bool(torch.isfinite(y[:r, 0, 3]).any()) and not bool(torch.isfinite(y[r - 1, 1, 5]))
+        rest = torch.ones_like(y, dtype=torch.bool)
+        rest[:r, 0, 3] = False
+        rest[:r, 1, 5] = False
+        assert torch.equal(y[rest], clean[0][rest])
+        dyb = dy.clone()
+        dyb[r, 1, 9] = bad                          # and a gradient behind the reset does not reach in front of it
+        df, dx, dh0, _ = hip.glr_backward(a["f"], x, dyb, saved, resets=a["resets"], bias=a["bias"])
+        assert torch.equal(dx[:r], gclean[1][:r]) and torch.equal(dh0, gclean[2])
+        assert torch.equal(df[r + 1:], gclean[0][r + 1:])
+    # a reset at the first step hides h0 as a whole
+    a["resets"][0] = 1
+    y0, _, s0 = hip.glr_forward(a["f"], a["x"], torch.full_like(a["h0"], float("nan")), resets=a["resets"], bias=a["bias"], want_saved=True)
+    assert bool(torch.isfinite(y0).all())
+    df, dx, dh0, db = hip.glr_backward(a["f"], a["x"], dy, s0, resets=a["resets"], bias=a["bias"])
+    assert bool((dh0 == 0).all()) and bool(torch.isfinite(df).all()) and bool(torch.isfinite(db).all())
+
+
+@pytest.mark.parametrize("T", [3, 50, 600])
+def test_gates_at_their_ends(hip, T):
+    """Gates that are fully open or shut, by infinities, by the type's ends and by sizes where exp leaves float32."""
+    ends = [float("inf"), -float("inf"), 3.4028234e38, -3.4028234e38, 200.0, -200.0, 90.0, -90.0, 30.0, -30.0, 17.0, -17.0, 0.0]
+    f = torch.tensor(ends, device="cuda").expand(T, 2, len(ends)).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(f.shape, generator=g, device="cuda") for _ in range(2))
+    h0 = torch.randn(2, len(ends), generator=g, device="cuda")
+    y, last, saved = hip.glr_forward(f, x, h0, want_saved=True)
+    want = ref.forward(f, x, h0)[0]
+    # worst case of the size of glr_reference.Bounds with K = T and gates 8 U off; f itself is exact here
+    tol = ref.U * 4.0 * (16 + 6 * T)
+    close(y, want, torch.full_like(want, tol), "y")
+    assert torch.equal(y[:, :, 0], h0[:, 0].expand(T, 2)) and torch.equal(y[:, :, 1], x[:, :, 1])
+    df, dx, dh0, _ = hip.glr_backward(f, x, dy, saved)
+    wf, wx, w0, _ = ref.backward(f, x, h0, None, None, dy)
+    top = ref.largest_g(f, None, None, dy, None)
+    tol = ref.U * top * (64 + 6 * T)
+    close(dx, wx, tol, "dx")
+    close(df, wf, 4 * tol, "df")
+    close(dh0, w0, tol, "dh0")
+
+
+@pytest.mark.parametrize("T", [4, 40, 600])
+def test_infinities_and_nans_follow_the_formula(hip, T):
+    f = torch.zeros(T, 1, 8, device="cuda")
+    x = torch.ones(T, 1, 8, device="cuda")
+    x[1, 0, 0], x[1, 0, 1], x[1, 0, 2] = float("inf"), -float("inf"), float("nan")
+    x[1, 0, 3], x[2, 0, 3] = float("inf"), -float("inf")
+    f[2, 0, 4] = float("nan")
+    x[1, 0, 5], x[2, 0, 5] = 3e38, -3e38            # a distance beyond float32
+    f[:, 0, 6] = 4.0
+    x[1, 0, 6] = float("inf")                       # kept by a gate next to one
+    f[:, 0, 7] = -4.0
+    x[1, 0, 7] = float("inf")
+    y, last, _ = hip.glr_forward(f, x)
+    want = ref.forward(f, x)[0].float()
+    assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.sign(y[~fin & ~torch.isnan(want)]), torch.sign(want[~fin & ~torch.isnan(want)]))
+    assert bool(((y[fin] - want[fin]).abs() <= 1e-5 * want[fin].abs() + 1e-5).all())        # K = 2: 28 U of the largest input of the column
+
+
+def test_long_memory(hip):
+    """Gates of 1 - 3e-6 over 20000 steps: a gate rounded to float32 would be off by 1 % of its distance to one.  The bound
+    counts one rounding of the state per span of 16 steps at random signs, not one per step: a straight sum of the worst case
+    says 20000 U = 1e-3, which the rounded gate would pass as well."""
+    T, H = 20000, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    f = torch.full((T, 1, H), 12.7, device="cuda")
+    x = 1 + 0.1 * torch.randn(T, 1, H, generator=g, device="cuda")
+    y, last, saved = hip.glr_forward(f, x, want_saved=True)
+    want = ref.forward(f, x)[0]
+    rel = ((y.double() - want).abs().amax((1, 2)) / want.abs().amax((1, 2)))[100:]
+    # 20000 roundings of at most U each, all the same way, against a state that grows to 6 %: 20000 U * (sum of the states so far
+    # over steps and the last state) <= 20000 U / 2 = 6e-4; at random signs sqrt(20000) U = 8.4e-6, six times that for the worst of 64 columns
+    assert float(rel.max()) < 5.1e-5, float(rel.max())
+    dy = torch.randn(T, 1, H, generator=g, device="cuda")
+    df, dx, dh0, _ = hip.glr_backward(f, x, dy, saved)
+    wf, wx, w0, _ = ref.backward(f, x, None, None, None, dy)
+    for got, w in ((df, wf), (dx, wx), (dh0, w0)):
+        assert float((got.double() - w).norm() / w.norm()) < 5.1e-5
+
+
+def test_nothing_to_do(hip):
+    z = lambda *s: torch.zeros(s, device="cuda")        # noqa: E731
+    h0 = torch.randn(3, 5, device="cuda")
+    y, last, saved = hip.glr_forward(z(0, 3, 5), z(0, 3, 5), h0, bias=z(5), want_saved=True)
+    assert y.shape == (0, 3, 5) and torch.equal(last, h0)
+    dl = torch.randn(3, 5, device="cuda")
+    df, dx, dh0, db = hip.glr_backward(z(0, 3, 5), z(0, 3, 5), z(0, 3, 5), saved, bias=z(5), dh_last=dl)
+    assert torch.equal(dh0, dl) and bool((db == 0).all()) and df.shape == (0, 3, 5)
+    assert bool((hip.glr_forward(z(0, 3, 5), z(0, 3, 5))[1] == 0).all())
+    for shape in ((4, 0, 5), (4, 3, 0)):
+        y, last, saved = hip.glr_forward(z(*shape), z(*shape), bias=z(shape[2]), want_saved=True)
+        assert y.shape == shape and last.shape == shape[1:]
+        df, dx, dh0, db = hip.glr_backward(z(*shape), z(*shape), z(*shape), saved, bias=z(shape[2]))
+        assert db.shape == (shape[2],) and bool((db == 0).all())
+    assert hip.glr_step(z(0, 5), z(0, 5), z(0, 5)).shape == (0, 5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_steps_follow_the_sequence(hip, dtype):
+    T, E, H = 40, 37, 129
+    a, _ = make(T, E, H, dtype, kind="joint", resets=True, bias=True)
+    want, last, _ = ref.forward(a["f"], a["x"], a["h0"], a["resets"], a["bias"])
+    tol = ref.Bounds(a["f"], a["x"], a["h0"], a["resets"], a["bias"]).h
+    state = a["h0"].clone()
+    out = torch.empty(E, H, dtype=dtype, device="cuda")
+    for t in range(T):
+        y = hip.glr_step(a["f"][t], a["x"][t], state, resets=a["resets"][t], bias=a["bias"], y=out if t % 2 else None)
+        assert (y is out) == bool(t % 2)
+        close(y, want[t], tol, "y[%d]" % t)
+    close(state, last, tol, "state")
+
+
+def test_state_may_be_none_of_the_outputs(hip):
+    s = torch.zeros(3, 8, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        hip.glr_step(torch.zeros(3, 8, device="cuda"), torch.zeros(3, 8, device="cuda"), s, y=s)
+    with pytest.raises(ValueError, match="overlaps"):
+        hip.glr_forward(torch.zeros(2, 3, 8, device="cuda"), torch.zeros(2, 3, 8, device="cuda"), h0=s, h_last=s)
+    with pytest.raises(TypeError, match="all tensors"):
+        hip.glr_forward(torch.zeros(2, 3, 8), torch.zeros(2, 3, 8, device="cuda"))
+
+
+@pytest.mark.parametrize("T,E,H", [(600, 2, 130), (5000, 1, 64), (20, 300, 64)])
+def test_same_bits_every_time(hip, T, E, H):
+    a, normal = make(T, E, H, BF16, resets=True, bias=True)
+    dy = normal(T, E, H).to(BF16)
+    first = None
+    for _ in range(3):
+        y, last, saved = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+        out = (y, last) + hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"])
+        first = first or out
+        assert all(torch.equal(p, q) for p, q in zip(first, out))
+
+
+def test_gradients_against_differences(hip):
+    """Directional differences of the GPU's own forward pass, summed in 64 bits: step 2^-7 leaves 6e-5 times third derivatives of
+    order one of a loss of 2000 terms at random signs, and float32 values of 2^-24 * 40 per term over the step."""
+    T, E, H = 50, 2, 20
+    a, normal = make(T, E, H, F32, bias=True, reach=2.0)
+    w, wl = normal(T, E, H), normal(E, H)
+
+    def loss(f, x, h0, b):
+        y, last, _ = hip.glr_forward(f, x, h0, bias=b)
+        return float((y.double() * w).sum() + (last.double() * wl).sum())
+
+    _, _, saved = hip.glr_forward(a["f"], a["x"], a["h0"], bias=a["bias"], want_saved=True)
+    df, dx, dh0, db = hip.glr_backward(a["f"], a["x"], w, saved, bias=a["bias"], dh_last=wl)
+    at = [a["f"], a["x"], a["h0"], a["bias"]]
+    for k, grad in enumerate((df, dx, dh0, db)):
+        v = torch.randn_like(at[k])
+        v /= v.norm()
+        up, down = ([q + s * v if i == k else q for i, q in enumerate(at)] for s in (2.0 ** -7, -2.0 ** -7))
+        diff = (loss(*up) - loss(*down)) * 2.0 ** 6
+        want = float((grad.double() * v).sum())
+        assert abs(diff - want) < 2e-2 * (1 + abs(want)), (k, diff, want)
+
+
+def test_another_stream(hip):
+    T, E, H = 400, 3, 200
+    a, normal = make(T, E, H, BF16, resets=True, bias=True)
+    dy = normal(T, E, H).to(BF16)
+    want = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    gwant = hip.glr_backward(a["f"], a["x"], dy, want[2], resets=a["resets"], bias=a["bias"])
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for s in (s1, s2, s1, s2):                     # calls that overlap in time share nothing
+        with torch.cuda.stream(s):
+            y, last, saved = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+            outs.append((y, last) + hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"]))
+    torch.cuda.synchronize()
+    for o in outs:
+        assert all(torch.equal(p, q) for p, q in zip(o, want[:2] + gwant))
+
+
+@pytest.mark.parametrize("T,E,H", [(1000, 1, 128), (40, 4, 64)])
+def test_captured_and_replayed(hip, T, E, H):
+    """Two graphs with their own workspaces, replayed in turn with eager work between, against eager results on new inputs."""
+    a, normal = make(T, E, H, F32, resets=True, bias=True)
+    dy = normal(T, E, H)
+    one = lambda: hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)       # noqa: E731
+
+    def both():
+        y, last, saved = one()
+        return (y, last) + hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"])
+    both()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = both()
+        graphs.append((g, outs))
+    for k in range(4):
+        for t in (a["f"], a["x"], a["h0"], dy):
+            t.copy_(torch.randn_like(t))
+        a["resets"].copy_(torch.rand(T, E, device="cuda") < 0.1)
+        want = both()
+        for g, outs in graphs:
+            for o in outs:
+                o.fill_(3.0)
+            g.replay()
+        graphs[k % 2][0].replay()
+        torch.cuda.synchronize()
+        for g, outs in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(outs, want)), k
+
+
+def test_offsets_beyond_32_bits(hip):
+    """Steps 2^31 + 40 elements apart (a bfloat16 buffer of 12.9 GB of which three rows are used)."""
+    T, E, H = 3, 2, 70
+    st = (1 << 31) + 40
+    buf = torch.empty((T - 1) * st + 400, dtype=BF16, device="cuda")
+    views = [buf.as_strided((T, E, H), (st, H, 1), k * 140) for k in range(2)]
+    a, normal = make(T, E, H, BF16, bias=True)
+    for v, t in zip(views, (a["f"], a["x"])):
+        v.copy_(t)
+    a["f"], a["x"] = views
+    check(hip, a, normal, BF16)
