@@ -15,7 +15,9 @@ constexpr int kBlock = PPO2HIP_ADAMW_BLOCK;      // elements of one scale
 constexpr int kChunk = 2048;                     // elements a workgroup takes at a time: 8 per thread, 8 blocks of 8-bit moments
 constexpr int kThreads = 256;
 constexpr int kMaxGrads = 448;                   // gradient pointers of one launch: they ride in its 4 KB of arguments
-constexpr int kNormGroups = 1024;                // workgroups of the norm launch = partial sums every workgroup of the step adds up
+constexpr int kNormGroups = 4096;                // most workgroups of the norm launch, each with a partial sum
+constexpr int kOwnSums = 512;                    // most partial sums that every workgroup of the step adds up by itself
+constexpr int kOwnChunks = 2048;                 // chunks from which it does not
 
 struct TensorRow {                               // one tensor in the device image of a plan
     void *p;
@@ -36,9 +38,10 @@ struct AdamwArgs {
     void *m, *v;
     float *m_scale, *v_scale;
     const double *partial;
-    int32_t npartial;
+    int32_t npartial;                            // 0: the factor stands in norm_out[1] already
     float lr, c1, c2, b1, b2, omb1, omb2, eps, wd, gscale, max_norm;
     float *norm_out;
+    const float *factor;
     const void *g[kMaxGrads];
 };
 static_assert(sizeof(AdamwArgs) <= 4096, "arguments beyond what a launch carries");
@@ -63,11 +66,13 @@ __device__ inline f32x4 load4(const void *base, int type, int64_t i, int64_t n) 
     if (type == PPO2HIP_F32) {
         const float *p = (const float *)base + i;
         if (i + 4 <= n) return *(const f32x4_any *)p;
+#pragma unroll
         for (int k = 0; k < 3; k++)
             if (i + k < n) r[k] = p[k];
     } else {
         const __bf16 *p = (const __bf16 *)base + i;
         if (i + 4 <= n) return __builtin_convertvector(*(const bf16x4_any *)p, f32x4);
+#pragma unroll
         for (int k = 0; k < 3; k++)
             if (i + k < n) r[k] = (float)p[k];
     }
@@ -80,12 +85,14 @@ __device__ inline void store4(void *base, int type, int64_t i, int64_t n, f32x4 
         float *p = (float *)base + i;
         if (i + 4 <= n) *(f32x4_any *)p = v;
         else
+#pragma unroll
             for (int k = 0; k < 3; k++)
                 if (i + k < n) p[k] = v[k];
     } else {
         __bf16 *p = (__bf16 *)base + i;
         if (i + 4 <= n) *(bf16x4_any *)p = __builtin_convertvector(v, bf16x4);
         else
+#pragma unroll
             for (int k = 0; k < 3; k++)
                 if (i + k < n) p[k] = (__bf16)v[k];
     }
@@ -102,28 +109,53 @@ __device__ inline float square_of(uint8_t c, float scale) {
     return scale * (x * x * (1.f / 4228250625.f));
 }
 
+constexpr int kParts = kChunk / (4 * kThreads);      // four-element parts of a chunk that a thread has
+
 __global__ __launch_bounds__(kThreads) void adamw_norm_kernel(NormArgs a) {
     __shared__ double red[17];
     double s = 0.0;
     for (int c = blockIdx.x; c < a.nchunks; c += gridDim.x) {
         const ChunkRow ch = a.chunks[c];
-        const void *g = a.g[ch.tensor - a.first_tensor];
-        if (!g) continue;
         const TensorRow &t = a.tensors[ch.tensor];
+        const void *g = a.g[ch.tensor - a.first_tensor];
+        if (g) {
+            f32x4 x[kParts];
 #pragma unroll
-        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
-            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
-            if (i >= t.n) break;
-            const f32x4 x = load4(g, t.g_type, i, t.n);
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const double d = (double)(x[k] * a.gscale);
-                s += d * d;                       // in 64 bits: squares of float32 leave its range
+            for (int u = 0; u < kParts; u++) {
+                const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
+                x[u] = load4(g, t.g_type, i, t.n);
             }
+#pragma unroll
+            for (int u = 0; u < kParts; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const double d = (double)(x[u][k] * a.gscale);
+                    s += d * d;                   // in 64 bits: squares of float32 leave its range
+                }
         }
     }
     s = block_sum(s, red);
     if (threadIdx.x == 0) a.partial[blockIdx.x] = s;
+}
+
+__device__ inline float norm_of(const double *partial, int n, double *red) {
+    double s = 0.0;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) s += partial[i];
+    return (float)sqrt(block_sum(s, red));
+}
+// not fmaxf: a norm that is not a number stays one
+__device__ inline float factor_of(float norm, float gscale, float max_norm) {
+    return gscale * (norm > max_norm ? max_norm / norm : (norm <= max_norm ? 1.f : norm));
+}
+// {norm, factor} for lists of many chunks: one workgroup adds up what every workgroup of the step would have to
+__global__ __launch_bounds__(1024) void adamw_factor_kernel(const double *partial, int npartial, float gscale, float max_norm, float *factor, float *norm_out) {
+    __shared__ double red[17];
+    const float norm = norm_of(partial, npartial, red);
+    if (threadIdx.x == 0) {
+        factor[0] = norm;
+        factor[1] = factor_of(norm, gscale, max_norm);
+        if (norm_out) norm_out[0] = norm, norm_out[1] = factor[1];
+    }
 }
 
 __device__ inline unsigned wave_umax(unsigned v) {
@@ -135,94 +167,115 @@ __device__ inline unsigned wave_umax(unsigned v) {
     return v;
 }
 
+// The codes of a wave's block of 256, four elements to a lane, and their scale: the largest bit pattern, so that an infinity or
+// a NaN wins over every finite value; its block then decodes to NaN instead of to something that looks sound.  Roots of the
+// ratio to the scale, by the hardware's root (off by 2^-23 of its value, of a code's place by 3e-5 of a step at most).
+template <int ROOT>
+__device__ inline unsigned encode(const f32x4 &v, float &scale) {
+    constexpr float kTop = ROOT == 2 ? 127.f : 255.f;
+    unsigned top = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const unsigned x = __float_as_uint(v[k]) & 0x7fffffffu;
+        top = top > x ? top : x;
+    }
+    top = wave_umax(top);
+    const bool sound = top < 0x7f800000u;
+    scale = sound ? __uint_as_float(top) : __builtin_nanf("");
+    // a scale whose reciprocal would leave float32 is lifted together with its block
+    const float lift = scale < 0x1p-100f ? 0x1p120f : 1.f, inv = scale > 0.f ? 1.f / (scale * lift) : 0.f;
+    unsigned codes = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float ratio = sound ? fabsf(v[k]) * lift * inv : 0.f;
+        float root = __builtin_amdgcn_sqrtf(ratio);
+        if (ROOT == 4) root = __builtin_amdgcn_sqrtf(root);
+        int c = (int)rintf(root * kTop);
+        c = c < (int)kTop ? c : (int)kTop;
+        if (ROOT == 4) {
+            if (sound && v[k] > 0.f && c == 0) c = 1;
+        } else {
+            c = v[k] < 0.f ? -c : c;
+        }
+        codes |= (unsigned)(c & 255) << (8 * k);
+    }
+    return codes;
+}
+
 template <int BITS>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(AdamwArgs a) {
     __shared__ double red[17];
     float scale = a.gscale;
-    if (a.max_norm > 0.f) {
-        double s = 0.0;
-        for (int i = threadIdx.x; i < a.npartial; i += kThreads) s += a.partial[i];
-        s = block_sum(s, red);
-        const float norm = (float)sqrt(s);
-        // not fmaxf: a norm that is not a number stays one
-        scale = a.gscale * (norm > a.max_norm ? a.max_norm / norm : (norm <= a.max_norm ? 1.f : norm));
-        if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[0] = norm;
+    if (a.max_norm > 0.f && a.npartial == 0) {
+        scale = a.factor[1];
+    } else {
+        if (a.max_norm > 0.f) {
+            const float norm = norm_of(a.partial, a.npartial, red);
+            scale = factor_of(norm, a.gscale, a.max_norm);
+            if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[0] = norm;
+        }
+        if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[1] = scale;
     }
-    if (a.norm_out && blockIdx.x == 0 && threadIdx.x == 0) a.norm_out[1] = scale;
 
     for (int c = blockIdx.x; c < a.nchunks; c += gridDim.x) {
         const ChunkRow ch = a.chunks[c];
-        const void *gp = a.g[ch.tensor - a.first_tensor];
-        if (!gp) continue;
         const TensorRow t = a.tensors[ch.tensor];
+        const void *gp = a.g[ch.tensor - a.first_tensor];
         const float wd = a.wd * t.decay;
+        const int64_t i0 = (int64_t)ch.index * kChunk + threadIdx.x * 4;
+        if (gp) {
+            f32x4 g[kParts], p[kParts], m[kParts], v[kParts];
+            unsigned mc[kParts], vc[kParts];
+            float sm[kParts], sv[kParts];
 #pragma unroll
-        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
-            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
-            if ((BITS == 32 ? i : i - (threadIdx.x & 63) * 4) >= t.n) break;      // 8 bits: a wave works on its block as a whole
-            f32x4 g = {0.f, 0.f, 0.f, 0.f}, p = g, m = g, v = g;
-            if (i < t.n) {
-                g = load4(gp, t.g_type, i, t.n);
-                p = load4(t.p, t.p_type, i, t.n);
-            }
-            float sm = 0.f, sv = 0.f;
-            const int64_t blk = (t.off + i) / kBlock;
-            if (BITS == 32) {
-                m = load4((const float *)a.m + t.off, PPO2HIP_F32, i, t.n);
-                v = load4((const float *)a.v + t.off, PPO2HIP_F32, i, t.n);
-            } else {
-                const unsigned mc = ((const unsigned *)a.m)[(t.off + i) / 4], vc = ((const unsigned *)a.v)[(t.off + i) / 4];
-                sm = a.m_scale[blk];
-                sv = a.v_scale[blk];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    m[k] = moment_of((int8_t)(mc >> (8 * k)), sm);
-                    v[k] = square_of((uint8_t)(vc >> (8 * k)), sv);
+            for (int u = 0; u < kParts; u++) {
+                const int64_t i = i0 + u * (4 * kThreads);
+                g[u] = load4(gp, t.g_type, i, t.n);
+                p[u] = load4(t.p, t.p_type, i, t.n);
+                if (BITS == 32) {
+                    m[u] = load4((const float *)a.m + t.off, PPO2HIP_F32, i, t.n);
+                    v[u] = load4((const float *)a.v + t.off, PPO2HIP_F32, i, t.n);
+                } else {
+                    mc[u] = vc[u] = 0;
+                    sm[u] = sv[u] = 0.f;
+                    if (i - (threadIdx.x & 63) * 4 < t.n) {            // whole blocks: the codes reach to a block's end
+                        mc[u] = ((const unsigned *)a.m)[(t.off + i) / 4];
+                        vc[u] = ((const unsigned *)a.v)[(t.off + i) / 4];
+                        sm[u] = a.m_scale[(t.off + i) / kBlock];
+                        sv[u] = a.v_scale[(t.off + i) / kBlock];
+                    }
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const float gs = g[k] * scale;
-                m[k] = a.b1 * m[k] + a.omb1 * gs;
-                v[k] = a.b2 * v[k] + a.omb2 * (gs * gs);
-                p[k] = p[k] - a.lr * (m[k] * a.c1 / (sqrtf(v[k] * a.c2) + a.eps) + wd * p[k]);
-            }
-            if (i < t.n) store4(t.p, t.p_type, i, t.n, p);
-            if (BITS == 32) {
-                store4((float *)a.m + t.off, PPO2HIP_F32, i, t.n, m);
-                store4((float *)a.v + t.off, PPO2HIP_F32, i, t.n, v);
-            } else {
-                // largest bit patterns: an infinity or a NaN of the block wins over every finite value, its scale becomes the
-                // block's scale and the block decodes to NaN instead of to something that looks sound
-                unsigned um = 0, uv = 0;
+            for (int u = 0; u < kParts; u++) {
+                const int64_t i = i0 + u * (4 * kThreads);
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    if (i + k >= t.n) m[k] = 0.f, v[k] = 0.f;
-                    const unsigned x = __float_as_uint(m[k]) & 0x7fffffffu, y = __float_as_uint(v[k]) & 0x7fffffffu;
-                    um = um > x ? um : x;
-                    uv = uv > y ? uv : y;
+                    if (BITS == 8) {
+                        m[u][k] = moment_of((int8_t)(mc[u] >> (8 * k)), sm[u]);
+                        v[u][k] = square_of((uint8_t)(vc[u] >> (8 * k)), sv[u]);
+                    }
+                    const float gs = g[u][k] * scale;
+                    m[u][k] = a.b1 * m[u][k] + a.omb1 * gs;
+                    v[u][k] = a.b2 * v[u][k] + a.omb2 * (gs * gs);
+                    p[u][k] = p[u][k] - a.lr * (m[u][k] * a.c1 / (sqrtf(v[u][k] * a.c2) + a.eps) + wd * p[u][k]);
+                    if (BITS == 8 && i + k >= t.n) m[u][k] = 0.f, v[u][k] = 0.f;
                 }
-                um = wave_umax(um);
-                uv = wave_umax(uv);
-                const bool sound_m = um < 0x7f800000u, sound_v = uv < 0x7f800000u;
-                sm = sound_m ? __uint_as_float(um) : __builtin_nanf("");
-                sv = sound_v ? __uint_as_float(uv) : __builtin_nanf("");
-                const float im = sm > 0.f ? 127.f / sqrtf(sm) : 0.f, iv = sv > 0.f ? 255.f / sqrtf(sqrtf(sv)) : 0.f;
-                unsigned mc = 0, vc = 0;
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const float x = sound_m ? rintf(sqrtf(fabsf(m[k])) * im) : 0.f, y = sound_v ? rintf(sqrtf(sqrtf(v[k])) * iv) : 0.f;
-                    int cm = (int)fminf(x, 127.f), cv = (int)fminf(y, 255.f);
-                    if (cv == 0 && sound_v && v[k] > 0.f) cv = 1;
-                    cm = m[k] < 0.f ? -cm : cm;
-                    mc |= (unsigned)(cm & 255) << (8 * k);
-                    vc |= (unsigned)cv << (8 * k);
-                }
-                ((unsigned *)a.m)[(t.off + i) / 4] = mc;
-                ((unsigned *)a.v)[(t.off + i) / 4] = vc;
-                if ((threadIdx.x & 63) == 0) {
-                    a.m_scale[blk] = sm;
-                    a.v_scale[blk] = sv;
+                if (i < t.n) store4(t.p, t.p_type, i, t.n, p[u]);
+                if (BITS == 32) {
+                    if (i < t.n) {
+                        store4((float *)a.m + t.off, PPO2HIP_F32, i, t.n, m[u]);
+                        store4((float *)a.v + t.off, PPO2HIP_F32, i, t.n, v[u]);
+                    }
+                } else if (i - (threadIdx.x & 63) * 4 < t.n) {
+                    mc[u] = encode<2>(m[u], sm[u]);
+                    vc[u] = encode<4>(v[u], sv[u]);
+                    ((unsigned *)a.m)[(t.off + i) / 4] = mc[u];
+                    ((unsigned *)a.v)[(t.off + i) / 4] = vc[u];
+                    if ((threadIdx.x & 63) == 0) {
+                        a.m_scale[(t.off + i) / kBlock] = sm[u];
+                        a.v_scale[(t.off + i) / kBlock] = sv[u];
+                    }
                 }
             }
         }
@@ -234,25 +287,34 @@ template <class T>
 __global__ __launch_bounds__(kThreads) void adamw_state_kernel(const TensorRow *tensors, const ChunkRow *chunks, const int64_t *packed, int nchunks,
                                                                const unsigned *mc_, const unsigned *vc_, const float *m_scale, const float *v_scale,
                                                                T *m_out, T *v_out) {
+    const int type = sizeof(T) == 4 ? PPO2HIP_F32 : PPO2HIP_BF16;
     for (int c = blockIdx.x; c < nchunks; c += gridDim.x) {
         const ChunkRow ch = chunks[c];
-        const TensorRow &t = tensors[ch.tensor];
-        const int64_t at = packed[ch.tensor];
+        const TensorRow t = tensors[ch.tensor];
+        const int64_t at = packed[ch.tensor], i0 = (int64_t)ch.index * kChunk + threadIdx.x * 4;
+        unsigned mc[kParts], vc[kParts];
+        float sm[kParts], sv[kParts];
 #pragma unroll
-        for (int u = 0; u < kChunk / (4 * kThreads); u++) {
-            const int64_t i = (int64_t)ch.index * kChunk + u * (4 * kThreads) + threadIdx.x * 4;
-            if (i >= t.n) break;
-            const unsigned mc = mc_[(t.off + i) / 4], vc = vc_[(t.off + i) / 4];
-            const float sm = m_scale[(t.off + i) / kBlock], sv = v_scale[(t.off + i) / kBlock];
-            f32x4 m, v;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                m[k] = moment_of((int8_t)(mc >> (8 * k)), sm);
-                v[k] = square_of((uint8_t)(vc >> (8 * k)), sv);
+        for (int u = 0; u < kParts; u++) {
+            const int64_t i = i0 + u * (4 * kThreads);
+            if (i < t.n) {
+                mc[u] = mc_[(t.off + i) / 4], vc[u] = vc_[(t.off + i) / 4];
+                sm[u] = m_scale[(t.off + i) / kBlock], sv[u] = v_scale[(t.off + i) / kBlock];
             }
-            const int type = sizeof(T) == 4 ? PPO2HIP_F32 : PPO2HIP_BF16;
-            store4(m_out + at, type, i, t.n, m);
-            store4(v_out + at, type, i, t.n, v);
+        }
+#pragma unroll
+        for (int u = 0; u < kParts; u++) {
+            const int64_t i = i0 + u * (4 * kThreads);
+            if (i < t.n) {
+                f32x4 m, v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    m[k] = moment_of((int8_t)(mc[u] >> (8 * k)), sm[u]);
+                    v[k] = square_of((uint8_t)(vc[u] >> (8 * k)), sv[u]);
+                }
+                store4(m_out + at, type, i, t.n, m);
+                store4(v_out + at, type, i, t.n, v);
+            }
         }
     }
 }
@@ -332,7 +394,7 @@ extern "C" int ppo2hip_adamw_plan_fill(const ppo2hip_adamw_tensor *tensors, int 
 extern "C" size_t ppo2hip_adamw_workspace_bytes(const ppo2hip_adamw_tensor *tensors, int ntensors) {
     (void)tensors;
     const int64_t launches = ceil_div(ntensors > 0 ? ntensors : 1, kMaxGrads);
-    return (size_t)launches * kNormGroups * sizeof(double);
+    return 16 + (size_t)launches * kNormGroups * sizeof(double);
 }
 
 extern "C" int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, const void *plan, const void *const *grads,
@@ -359,8 +421,11 @@ extern "C" int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntens
     hipStream_t s = (hipStream_t)stream;
     const TensorRow *rows = (const TensorRow *)plan;
     const ChunkRow *chunks = (const ChunkRow *)((const char *)plan + shape.chunk_off);
-    double *partial = (double *)workspace;
+    float *factor = (float *)workspace;
+    double *partial = (double *)((char *)workspace + 16);
     int npartial = 0;
+    int64_t all_chunks = 0;
+    for (int k = 0; k < ntensors; k++) all_chunks += chunks_of(tensors[k].n);
     if (clip) {
         int64_t chunk = 0;
         for (int k0 = 0; k0 < ntensors; k0 += kMaxGrads) {
@@ -378,13 +443,20 @@ extern "C" int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntens
             a.nchunks = (int32_t)here;
             chunk += here;
             if (here == 0) continue;
-            const int groups = (int)(here < kNormGroups ? here : kNormGroups);
+            const int most = all_chunks <= kOwnChunks ? kOwnSums : kNormGroups;
+            const int groups = (int)(here < most ? here : most);
             hipLaunchKernelGGL(adamw_norm_kernel, dim3(groups), dim3(kThreads), 0, s, a);
             if ((rc = check_launch("adamw_norm_kernel"))) return rc;
             npartial += groups;
         }
     }
+    if (clip && all_chunks > kOwnChunks) {
+        hipLaunchKernelGGL(adamw_factor_kernel, dim3(1), dim3(1024), 0, s, partial, npartial, (float)grad_scale, (float)max_grad_norm, factor, norm_out);
+        if ((rc = check_launch("adamw_factor_kernel"))) return rc;
+        npartial = 0;
+    }
     AdamwArgs a;
+    a.factor = factor;
     a.tensors = rows;
     a.m = m;
     a.v = v;
@@ -416,7 +488,7 @@ extern "C" int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntens
         a.nchunks = (int32_t)here;
         chunk += here;
         if (here == 0) continue;
-        const int64_t groups = here < 2048 ? here : 2048;
+        const int64_t groups = here;
         if (state_bits == 32)
             hipLaunchKernelGGL(adamw_kernel<32>, dim3((unsigned)groups), dim3(kThreads), 0, s, a);
         else
@@ -440,7 +512,7 @@ extern "C" int ppo2hip_adamw_state(const ppo2hip_adamw_tensor *tensors, int nten
     const TensorRow *rows = (const TensorRow *)plan;
     const int64_t *packed = (const int64_t *)((const char *)plan + shape.packed_off);
     const ChunkRow *chunks = (const ChunkRow *)((const char *)plan + shape.chunk_off);
-    const unsigned groups = (unsigned)(nchunks < 4096 ? nchunks : 4096);
+    const unsigned groups = (unsigned)nchunks;
     hipStream_t s = (hipStream_t)stream;
     if (out_dtype == PPO2HIP_F32)
         hipLaunchKernelGGL(adamw_state_kernel<float>, dim3(groups), dim3(kThreads), 0, s, rows, chunks, packed, (int)nchunks, (const unsigned *)m,

@@ -211,7 +211,7 @@ using Span = float[kSpan][V];
 
 // A span's gates and what each step adds to the state, u = (1 - a) x.  Steps behind the last one keep the state as it is;
 // a step with a reset has its gate shut once u is formed, which multiplies a finite state by zero.
-template <class T, int V>
+template <class T, int V, bool BACK = false>
 __device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, unsigned rm, Span<V> &g, Span<V> &u) {
     typedef Gate<sizeof(T) == 4> G;
 #pragma unroll
@@ -219,7 +219,7 @@ __device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const f
 #pragma unroll
         for (int k = 0; k < V; k++) {
             g[i][k] = G::of((float)f.v[i][k] + b[k]);
-            u[i][k] = G::take(g[i][k]) * (float)x.v[i][k];
+            u[i][k] = BACK ? (float)x.v[i][k] : G::take(g[i][k]) * (float)x.v[i][k];
         }
     if (n < kSpan)
 #pragma unroll
@@ -283,16 +283,16 @@ __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run (&r)[V]) {
 }
 
 // The same against time, for the gradient: dy enters a step before the gate does, a reset stands behind it.
-template <class T, int V>
-__device__ inline void span_back(const Span<V> &g, const Raw<T, V> &dy, unsigned rm, Run (&r)[V]) {
-    typedef Gate<sizeof(T) == 4> G;
+template <bool EXACT, int V>
+__device__ inline void span_back(const Span<V> &g, const Span<V> &dy, unsigned rm, Run (&r)[V]) {
+    typedef Gate<EXACT> G;
     bool bad = false;
 #pragma unroll
     for (int k = 0; k < V; k++) r[k].B = 0.f;
 #pragma unroll
     for (int i = kSpan - 1; i >= 0; i--)
 #pragma unroll
-        for (int k = 0; k < V; k++) r[k].B = G::pass(g[i][k], r[k].B + (float)dy.v[i][k]);
+        for (int k = 0; k < V; k++) r[k].B = G::pass(g[i][k], r[k].B + dy[i][k]);
 #pragma unroll
     for (int k = 0; k < V; k++) bad |= !(fabsf(r[k].B) < INFINITY);
     if (__any(bad)) {
@@ -301,7 +301,7 @@ __device__ inline void span_back(const Span<V> &g, const Raw<T, V> &dy, unsigned
 #pragma unroll
         for (int i = kSpan - 1; i >= 0; i--)
 #pragma unroll
-            for (int k = 0; k < V; k++) r[k].B = rm >> i & 1 ? 0.f : G::pass_any(g[i][k], r[k].B + (float)dy.v[i][k]);
+            for (int k = 0; k < V; k++) r[k].B = rm >> i & 1 ? 0.f : G::pass_any(g[i][k], r[k].B + dy[i][k]);
     }
 }
 
@@ -363,21 +363,27 @@ __global__ __launch_bounds__(64 * kWaves) void glr_runs_kernel(Seq<const T> f, S
     Run r[V];
 #pragma unroll
     for (int k = 0; k < V; k++) b[k] = bias ? bias[at.j + k] : 0.f, r[k] = {1.f, 0.f, 0.f};
-    const int64_t first = ((int64_t)seg * kWaves + w) * cut.spans;
+    const int64_t first = ((int64_t)seg * kWaves + w) * cut.spans, last = (T_ + kSpan - 1) / kSpan;
+    const int64_t end = first + cut.spans < last ? first + cut.spans : last;
     Raw<T, V> fr, xr;
-    for (int i = 0; i < cut.spans; i++) {
-        const int64_t t0 = (first + (BACK ? cut.spans - 1 - i : i)) * kSpan;
-        if (t0 >= T_) continue;
+    auto fetch = [&](int64_t s) {
+        const int64_t t0 = s * kSpan;
         const int n = (int)(T_ - t0 < kSpan ? T_ - t0 : kSpan);
         fr.load(f, at, fo, t0, n);
         xr.load(x, at, xo, t0, n);
+    };
+    if (first < end) fetch(BACK ? end - 1 : first);
+    for (int64_t i = first; i < end; i++) {
+        const int64_t s = BACK ? end - 1 - (i - first) : i, t0 = s * kSpan;
+        const int n = (int)(T_ - t0 < kSpan ? T_ - t0 : kSpan);
         const unsigned rm = span_resets(resets, t0, n, at);
-        Span<V> g, u;
+        Span<V> g, u;                                       // BACK: u is dy
         Run one[V];
-        span_open<T, V>(fr, xr, b, n, rm, g, u);
+        span_open<T, V, BACK>(fr, xr, b, n, rm, g, u);
+        if (i + 1 < end) fetch(BACK ? s - 1 : s + 1);
         span_passes<sizeof(T) == 4, V>(g, rm, one);
         if (BACK) {
-            span_back<T, V>(g, xr, rm, one);
+            span_back<sizeof(T) == 4, V>(g, u, rm, one);
         } else {
             float h[V];
 #pragma unroll
@@ -636,7 +642,7 @@ __device__ inline void dbias_row(float *row, unsigned c, bool mine, int nw, cons
 }
 
 template <class T, int V>
-__global__ __launch_bounds__(64 * kWaves) void glr_backward_kernel(BackwardArgs<T> a, Shares cut) {
+__global__ __launch_bounds__(64 * kWaves, 2) void glr_backward_kernel(BackwardArgs<T> a, Shares cut) {
     __shared__ float part[kWaves][3][64 * V];
     __shared__ double sums[kWaves][64 * V];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seg = blockIdx.y;
@@ -705,12 +711,12 @@ __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardA
     back_open<T, V>(fr, xr, b, kept, n, rm, g, q);
     span_passes<sizeof(T) == 4, V>(g, rm, r);
     {
-        Span<V> shut;
+        Span<V> shut, dy;
 #pragma unroll
         for (int i = 0; i < kSpan; i++)
 #pragma unroll
-            for (int k = 0; k < V; k++) shut[i][k] = rm >> i & 1 ? Gate<sizeof(T) == 4>::shut() : g[i][k];
-        span_back<T, V>(shut, gr, rm, r);
+            for (int k = 0; k < V; k++) shut[i][k] = rm >> i & 1 ? Gate<sizeof(T) == 4>::shut() : g[i][k], dy[i][k] = (float)gr.v[i][k];
+        span_back<sizeof(T) == 4, V>(shut, dy, rm, r);
     }
 #pragma unroll
     for (int k = 0; k < V; k++) runs[w][0][lane * V + k] = r[k].A, runs[w][1][lane * V + k] = r[k].D, runs[w][2][lane * V + k] = r[k].B;
@@ -776,7 +782,8 @@ __global__ void glr_copy_state_kernel(const float *src, float *dst, int64_t n) {
 
 using namespace ppo2hip;
 
-constexpr int64_t kWaveTarget = 4096;
+constexpr int64_t kWaveTarget = 4096;     // waves that walk shares
+constexpr int64_t kAlone = 640;           // tiles from which a wave walks a whole sequence
 
 template <class T>
 static Seq<T> seq_of(const ppo2hip_seq *s) {
@@ -807,26 +814,29 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
     return ceil_div(T, kSpan) * (int64_t)E * H;
 }
 
-// How a call is cut: V channels per lane, tiles of 64 V columns, and the time axis held by one workgroup per tile, walked by
+// How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile, walked by
 // one wave per tile, or cut into shares.
 struct Cut {
-    int V, env_tiles;
-    int64_t tiles;
+    int V, run_V, env_tiles, run_env_tiles;     // run_*: of the launch that finds the shares' runs
+    int64_t tiles, run_tiles;
     bool held;
     Shares sh;
 };
-static Cut cut_of(int dtype, int T, int E, int H) {
+static Cut cut_of(int dtype, int T, int E, int H, bool back) {
     Cut k;
     const int64_t C = (int64_t)E * H, spans = ceil_div(T, kSpan);
-    k.V = dtype != PPO2HIP_F32 && H % 2 == 0 ? 2 : 1;
-    k.env_tiles = 0;
+    const int wide = dtype != PPO2HIP_F32 && H % 2 == 0 ? 2 : 1;
+    k.env_tiles = k.run_env_tiles = 0;
+    k.run_V = wide;
+    k.run_tiles = ceil_div(C, 64 * wide);
+    k.held = spans <= kHeld && k.run_tiles < kAlone;
+    // two channels per lane halve a 16-bit sequence's loads; the backward walk and the held spans have no registers for them
+    k.V = back || k.held ? 1 : wide;
     k.tiles = ceil_div(C, 64 * k.V);
-    int64_t want = ceil_div(kWaveTarget, k.tiles);
-    if (want > spans) want = spans;
-    k.held = want > 1 && spans <= kHeld;
-    if (k.held) k.V = 1, k.tiles = ceil_div(C, 64);         // 16 waves leave 128 registers to each: two channels per lane spill
     k.sh = Shares{(int)spans, 1, 1, nullptr, nullptr};
-    if (k.held || want <= 1) return k;
+    if (k.held || k.run_tiles >= kAlone) return k;
+    int64_t want = ceil_div(kWaveTarget, k.run_tiles);
+    if (want > spans) want = spans;
     k.sh.spans = (int)ceil_div(spans, want);
     k.sh.segs = (int)ceil_div(spans, (int64_t)k.sh.spans * kWaves);
     k.sh.shares = k.sh.segs * kWaves;
@@ -835,13 +845,15 @@ static Cut cut_of(int dtype, int T, int E, int H) {
 // Lanes of a tile in a row reach over up to 64 V / H envs behind the first: their offsets must fit 31 bits in every array,
 // else each env gets tiles of its own (lanes behind H idle there).
 static void place_envs(Cut &k, int E, int H, std::initializer_list<const ppo2hip_seq *> seqs) {
-    int64_t reach = (64 * k.V - 1) / H + 1;
+    int64_t reach = (64 * 2 - 1) / H + 1;
     if (reach > E - 1) reach = E - 1;
     bool far = false;
     for (const ppo2hip_seq *s : seqs) far |= s && reach > 0 && s->e > ((1ll << 29) - 1 - H) / reach;
     if (!far) return;
     k.env_tiles = (int)ceil_div(H, 64 * k.V);
+    k.run_env_tiles = (int)ceil_div(H, 64 * k.run_V);
     k.tiles = (int64_t)E * k.env_tiles;
+    k.run_tiles = (int64_t)E * k.run_env_tiles;
 }
 
 static size_t runs_bytes(const Cut &k, int64_t C) { return k.sh.shares > 1 ? align_up((size_t)(k.sh.segs + k.sh.shares) * 3 * C * sizeof(float), 256) : 0; }
@@ -852,16 +864,27 @@ static void place_runs(Cut &k, int64_t C, void *workspace) {
 
 extern "C" size_t ppo2hip_glr_forward_workspace_bytes(int dtype, int T, int E, int H) {
     if (T <= 1 || E <= 0 || H <= 0) return 0;
-    return runs_bytes(cut_of(dtype, T, E, H), (int64_t)E * H);
+    return runs_bytes(cut_of(dtype, T, E, H, false), (int64_t)E * H);
 }
 
 extern "C" size_t ppo2hip_glr_backward_workspace_bytes(int dtype, int T, int E, int H, int want_dbias) {
     if (T <= 0 || E <= 0 || H <= 0) return 0;
-    const Cut k = cut_of(dtype, T, E, H);
+    const Cut k = cut_of(dtype, T, E, H, true);
     const int64_t C = (int64_t)E * H, rows = (int64_t)k.sh.segs * E;
     size_t n = runs_bytes(k, C);
     if (want_dbias) n += align_up((size_t)rows * H * sizeof(float), 256) + align_up((size_t)ceil_div(rows, kSumRows) * H * sizeof(float), 256);
     return n;
+}
+
+template <class T, bool BACK>
+static int launch_runs(const Cut &k, const Seq<const T> &f, const Seq<const T> &x, const float *bias, const Seq<const uint8_t> &resets, int T_,
+                       unsigned C, unsigned H, hipStream_t s) {
+    const dim3 grid((unsigned)k.run_tiles, k.sh.segs), block(64 * kWaves);
+    if (sizeof(T) == 2 && k.run_V == 2)
+        hipLaunchKernelGGL((glr_runs_kernel<T, sizeof(T) == 2 ? 2 : 1, BACK>), grid, block, 0, s, f, x, bias, resets, T_, C, H, k.run_env_tiles, k.sh);
+    else
+        hipLaunchKernelGGL((glr_runs_kernel<T, 1, BACK>), grid, block, 0, s, f, x, bias, resets, T_, C, H, k.run_env_tiles, k.sh);
+    return check_launch("glr_runs_kernel");
 }
 
 template <class T, int V>
@@ -876,13 +899,11 @@ static int forward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, 
     const ForwardArgs<T> a = {seq_of<const T>(f), seq_of<const T>(x), seq_of<const uint8_t>(resets), seq_of<T>(y), bias, h0, h_last, saved,
                               T_, (unsigned)C, (unsigned)H, (unsigned)k.env_tiles};
     if (k.held) {
-        hipLaunchKernelGGL((glr_forward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
+        hipLaunchKernelGGL((glr_forward_held_kernel<T, 1>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
         return check_launch("glr_forward_held_kernel");
     }
     if (k.sh.shares > 1) {
-        hipLaunchKernelGGL((glr_runs_kernel<T, V, false>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * kWaves), 0, s, a.f, a.x, bias, a.resets,
-                           T_, a.C, a.H, a.env_tiles, k.sh);
-        int rc = check_launch("glr_runs_kernel");
+        int rc = launch_runs<T, false>(k, a.f, a.x, bias, a.resets, T_, a.C, a.H, s);
         if (rc) return rc;
     }
     hipLaunchKernelGGL((glr_forward_kernel<T, V>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * (k.sh.shares > 1 ? kWaves : 1)), 0, s, a, k.sh);
@@ -906,7 +927,7 @@ extern "C" int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip
         set_error("glr_forward: workspace of %zu bytes is too small", workspace_bytes);
         return PPO2HIP_ENOSPACE;
     }
-    Cut k = cut_of(dtype, T, E, H);
+    Cut k = cut_of(dtype, T, E, H, false);
     place_envs(k, E, H, {f, x, resets, y});
     PPO2HIP_REQUIRE(T == 1 || k.sh.shares == 1 || workspace, "glr_forward: workspace is null");
     place_runs(k, C, workspace);
@@ -930,11 +951,7 @@ static int backward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x,
         hipLaunchKernelGGL((glr_backward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
         rc = check_launch("glr_backward_held_kernel");
     } else {
-        if (k.sh.shares > 1) {
-            hipLaunchKernelGGL((glr_runs_kernel<T, V, true>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * kWaves), 0, s, a.f, a.dy, bias, a.resets,
-                               T_, a.C, a.H, a.env_tiles, k.sh);
-            if ((rc = check_launch("glr_runs_kernel"))) return rc;
-        }
+        if (k.sh.shares > 1 && (rc = launch_runs<T, true>(k, a.f, a.dy, bias, a.resets, T_, a.C, a.H, s))) return rc;
         hipLaunchKernelGGL((glr_backward_kernel<T, V>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * (k.sh.shares > 1 ? kWaves : 1)), 0, s, a, k.sh);
         rc = check_launch("glr_backward_kernel");
     }
@@ -973,13 +990,13 @@ extern "C" int ppo2hip_glr_backward(int dtype, int T, int E, int H, const ppo2hi
         set_error("glr_backward: workspace of %zu bytes is too small", workspace_bytes);
         return PPO2HIP_ENOSPACE;
     }
-    Cut k = cut_of(dtype, T, E, H);
+    Cut k = cut_of(dtype, T, E, H, true);
     place_envs(k, E, H, {f, x, resets, dy, df, dx});
     PPO2HIP_REQUIRE((!dbias && k.sh.shares == 1) || workspace, "glr_backward: workspace is null");
     place_runs(k, C, workspace);
-#define PPO2HIP_GLR_BACKWARD(type, V) backward_of<type, V>(k, f, x, bias, resets, saved, dy, dh_last, df, dx, dbias, dh0, workspace, T, E, H, s)
-    if (dtype == PPO2HIP_F32) return PPO2HIP_GLR_BACKWARD(float, 1);
-    if (dtype == PPO2HIP_BF16) return k.V == 2 ? PPO2HIP_GLR_BACKWARD(__bf16, 2) : PPO2HIP_GLR_BACKWARD(__bf16, 1);
-    return k.V == 2 ? PPO2HIP_GLR_BACKWARD(_Float16, 2) : PPO2HIP_GLR_BACKWARD(_Float16, 1);
+#define PPO2HIP_GLR_BACKWARD(type) backward_of<type, 1>(k, f, x, bias, resets, saved, dy, dh_last, df, dx, dbias, dh0, workspace, T, E, H, s)
+    if (dtype == PPO2HIP_F32) return PPO2HIP_GLR_BACKWARD(float);
+    if (dtype == PPO2HIP_BF16) return PPO2HIP_GLR_BACKWARD(__bf16);
+    return PPO2HIP_GLR_BACKWARD(_Float16);
 #undef PPO2HIP_GLR_BACKWARD
 }

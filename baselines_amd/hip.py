@@ -15,6 +15,12 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _raw_stream(index):
+    """The current stream of GPU ``index`` as a number: a thirtieth of what building a Stream object costs, which shows in
+    calls of a few microseconds."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _ptr(t):
     if t is None:
         return None
@@ -157,7 +163,7 @@ def _glr_f32(t, name, shape):
         raise TypeError("%s must be a float32 tensor" % name)
     if t.shape != shape or not t.is_contiguous():
         raise ValueError("%s must be contiguous with shape %s" % (name, tuple(shape)))
-    return ctypes.c_void_p(t.data_ptr())
+    return t.data_ptr()
 
 
 def _extent(t):
@@ -241,22 +247,18 @@ def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want
             return glr_forward(f, x, h0, resets, bias, y, h_last, want_saved)
     T, E, H = shape
     if y is None:
-        y = torch.empty(shape, dtype=dt, device=x.device)
+        y = x.new_empty(shape)
     if h_last is None:
-        h_last = torch.empty((E, H), dtype=torch.float32, device=x.device)
-    saved = None
-    if want_saved:
-        saved = GlrSaved(torch.empty((-(-T // _lib.GLR_SPAN), E, H), dtype=torch.float32, device=x.device), shape, dt)
-    _glr_call_forward(_GLR_TYPES[dt], T, E, H, sf, sx, pb, sr, p0, _lib.Seq(y.data_ptr(), *y.stride()[:2]), h_last,
-                      saved.states if saved else None, "glr_forward")
-    return y, h_last, saved
-
-
-def _glr_call_forward(code, T, E, H, f, x, bias, resets, h0, y, h_last, saved, what):
+        h_last = x.new_empty((E, H), dtype=torch.float32)
+    states = x.new_empty((-(-T // _lib.GLR_SPAN), E, H), dtype=torch.float32) if want_saved else None
+    code = _GLR_TYPES[dt]
     need = lib.ppo2hip_glr_forward_workspace_bytes(code, T, E, H)
-    ws = torch.empty(need, dtype=torch.uint8, device=h_last.device) if need else None
-    check(lib.ppo2hip_glr_forward(code, T, E, H, f, x, bias, resets, h0, y, h_last.data_ptr(), _ptr(saved), _ptr(ws), need, _stream()),
-          what)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    st, se, _ = y.stride()
+    check(lib.ppo2hip_glr_forward(code, T, E, H, sf, sx, pb, sr, p0, _lib.Seq(y.data_ptr(), st, se), h_last.data_ptr(),
+                                  states.data_ptr() if want_saved else None, ws.data_ptr() if need else None, need,
+                                  _raw_stream(x.device.index)), "glr_forward")
+    return y, h_last, GlrSaved(states, shape, dt) if want_saved else None
 
 
 def glr_step(f, x, state, resets=None, bias=None, y=None):
@@ -264,23 +266,12 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
     in place.  Returns y [E, H] in x's type."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _GLR_TYPES:
         raise TypeError("x must be a float32, bfloat16 or float16 tensor [E, H]")
-    if not isinstance(f, torch.Tensor) or f.dim() != 2:
-        raise TypeError("f must be a tensor [E, H]")
-    E, H = x.shape
-    shape, dt = (1, E, H), x.dtype
-    seqs = []
-    for t, name in ((f, "f"), (x, "x")) if y is None else ((f, "f"), (x, "x"), (y, "y")):
-        if not isinstance(t, torch.Tensor) or t.dtype != dt:
-            raise TypeError("%s must be a %s tensor" % (name, dt))
-        if t.shape != x.shape:
-            raise ValueError("%s must have shape %s, got %s" % (name, tuple(x.shape), tuple(t.shape)))
-        se, sj = t.stride()
-        if sj != 1 and H > 1:
-            raise ValueError("%s must be contiguous over its last dimension" % name)
-        seqs.append(_lib.Seq(t.data_ptr(), 0, se))
+    shape, dt = x.shape, x.dtype
+    E, H = shape
+    sf, sx = _glr_row(f, "f", shape, dt), _glr_row(x, "x", shape, dt)
+    pb, ps, sr = _glr_f32(bias, "bias", (H,)), _glr_f32(state, "state", shape), None
     if state is None:
         raise TypeError("state must be a float32 tensor")
-    pb, ps, sr = _glr_f32(bias, "bias", (H,)), _glr_f32(state, "state", (E, H)), None
     if resets is not None:
         if not isinstance(resets, torch.Tensor) or resets.dtype not in (torch.bool, torch.uint8):
             raise TypeError("resets must be a bool or uint8 tensor")
@@ -288,15 +279,29 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
             raise ValueError("resets must have shape %s, got %s" % ((E,), tuple(resets.shape)))
         sr = _lib.Seq(resets.data_ptr(), 0, resets.stride(0))
     if y is not None:
+        sy = _glr_row(y, "y", shape, dt)
         _glr_apart(y.unsqueeze(0), "y", (("f", f.unsqueeze(0)), ("x", x.unsqueeze(0)), ("state", state), ("resets", resets), ("bias", bias)))
     if _same_gpu(x, "x", (f, bias, resets, state, y)):
         with torch.cuda.device(x.device):
             return glr_step(f, x, state, resets, bias, y)
     if y is None:
-        y = torch.empty((E, H), dtype=dt, device=x.device)
-        seqs.append(_lib.Seq(y.data_ptr(), 0, H))
-    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, seqs[0], seqs[1], pb, sr, ps, seqs[2], ps, None, None, 0, _stream()), "glr_step")
+        y = x.new_empty(shape)
+        sy = _lib.Seq(y.data_ptr(), 0, H)
+    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, sf, sx, pb, sr, ps, sy, ps, None, None, 0, _raw_stream(x.device.index)),
+          "glr_step")
     return y
+
+
+def _glr_row(t, name, shape, dtype):
+    """[E, H] tensor with a contiguous last dimension, as one step of a sequence."""
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError("%s must be a %s tensor" % (name, dtype))
+    if t.shape != shape:
+        raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    se, sj = t.stride()
+    if sj != 1 and shape[1] > 1:
+        raise ValueError("%s must be contiguous over its last dimension" % name)
+    return _lib.Seq(t.data_ptr(), 0, se)
 
 
 def glr_backward(f, x, dy, saved, resets=None, bias=None, dh_last=None, df=None, dx=None):
@@ -324,19 +329,20 @@ def glr_backward(f, x, dy, saved, resets=None, bias=None, dh_last=None, df=None,
         with torch.cuda.device(x.device):
             return glr_backward(f, x, dy, saved, resets, bias, dh_last, df, dx)
     T, E, H = shape
-    dev = x.device
     if df is None:
-        df = torch.empty(shape, dtype=dt, device=dev)
+        df = x.new_empty(shape)
     if dx is None:
-        dx = torch.empty(shape, dtype=dt, device=dev)
-    dh0 = torch.empty((E, H), dtype=torch.float32, device=dev)
-    dbias = None if bias is None else torch.empty(H, dtype=torch.float32, device=dev)
+        dx = x.new_empty(shape)
+    dh0 = x.new_empty((E, H), dtype=torch.float32)
+    dbias = None if bias is None else x.new_empty(H, dtype=torch.float32)
     code = _GLR_TYPES[dt]
     need = lib.ppo2hip_glr_backward_workspace_bytes(code, T, E, H, int(bias is not None))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    check(lib.ppo2hip_glr_backward(code, T, E, H, sf, sx, pb, sr, saved.states.data_ptr(), sdy, pl, _lib.Seq(df.data_ptr(), *df.stride()[:2]),
-                                   _lib.Seq(dx.data_ptr(), *dx.stride()[:2]), _ptr(dbias), dh0.data_ptr(), _ptr(ws), need, _stream()),
-          "glr_backward")
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    ft, fe, _ = df.stride()
+    xt, xe, _ = dx.stride()
+    check(lib.ppo2hip_glr_backward(code, T, E, H, sf, sx, pb, sr, saved.states.data_ptr(), sdy, pl, _lib.Seq(df.data_ptr(), ft, fe),
+                                   _lib.Seq(dx.data_ptr(), xt, xe), None if bias is None else dbias.data_ptr(), dh0.data_ptr(),
+                                   ws.data_ptr() if need else None, need, _raw_stream(x.device.index)), "glr_backward")
     return df, dx, dh0, dbias
 
 
@@ -1036,25 +1042,24 @@ class AdamWPlan:
             self._ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=dev)
             self.norm = torch.zeros(2, dtype=torch.float32, device=dev)
         self._grads = (ctypes.c_void_p * n)()
-        self._fixed = tuple(_ptr(t) for t in (self._image, self.m, self.m_scale, self.v, self.v_scale, self.norm, self._ws))
+        self._fixed = tuple(None if t is None else t.data_ptr() for t in (self._image, self.m, self.m_scale, self.v, self.v_scale, self.norm,
+                                                                         self._ws))
 
-    def _grad_ptrs(self, grads):
+    def _check_grads(self, grads):
+        """One gradient or None per tensor -> the array of their addresses that the library call takes."""
         if len(grads) != len(self._ptrs):
             raise ValueError("adamw_step needs one gradient (or None) per tensor: %d for %d" % (len(grads), len(self._ptrs)))
-        ptrs, dev = self._grads, self.device
-        for k, g in enumerate(grads):
-            if g is None:
-                ptrs[k] = None
-                continue
-            if g.dtype != self.grad_dtypes[k] or g.device != dev:
-                raise TypeError("grads[%d] must be %s on %s" % (k, self.grad_dtypes[k], dev))
-            if g.numel() != self._numels[k] or not g.is_contiguous():
-                raise ValueError("grads[%d] must be contiguous with %d entries" % (k, self._numels[k]))
-            ptrs[k] = g.data_ptr() or None
-        for k, p in enumerate(self.params):
-            if p.data_ptr() != self._ptrs[k]:
-                raise ValueError("params[%d] has moved since the plan was made" % k)
-        return ptrs
+        gpu = self.device.index
+        for g, dt, n in zip(grads, self.grad_dtypes, self._numels):
+            if g is not None and not (g.dtype is dt and g.get_device() == gpu and g.numel() == n and g.is_contiguous()):
+                k = next(i for i, h in enumerate(grads) if h is g)
+                if g.dtype is not dt or g.get_device() != gpu:
+                    raise TypeError("grads[%d] must be %s on %s" % (k, dt, self.device))
+                raise ValueError("grads[%d] must be contiguous with %d entries" % (k, n))
+        if [p.data_ptr() for p in self.params] != self._ptrs:
+            raise ValueError("a tensor of the list has moved since the plan was made")
+        self._grads[:] = [g if g is None else g.data_ptr() or None for g in grads]
+        return self._grads
 
 
 def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, max_grad_norm=0.0, grad_scale=1.0):
@@ -1065,10 +1070,11 @@ def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_
     if plan.device.index != torch.cuda.current_device():
         with torch.cuda.device(plan.device):
             return adamw_step(plan, grads, lr, t, beta1, beta2, epsilon, weight_decay, max_grad_norm, grad_scale)
-    ptrs = plan._grad_ptrs(grads)
+    ptrs = plan._check_grads(grads)
     image, m, ms, v, vs, norm, ws = plan._fixed
     check(lib.ppo2hip_adamw_step(plan._tensors, len(ptrs), plan.state_bits, image, ptrs, m, ms, v, vs, lr, t, beta1, beta2, epsilon,
-                                 weight_decay, grad_scale, max_grad_norm or 0.0, norm, ws, plan._ws_bytes, _stream()), "adamw_step")
+                                 weight_decay, grad_scale, max_grad_norm or 0.0, norm, ws, plan._ws_bytes,
+                                 _raw_stream(plan.device.index)), "adamw_step")
 
 
 def adamw_state(plan, dtype=torch.float32):
@@ -1081,10 +1087,10 @@ def adamw_state(plan, dtype=torch.float32):
     if plan.device.index != torch.cuda.current_device():
         with torch.cuda.device(plan.device):
             return adamw_state(plan, dtype)
-    m, v = (torch.empty(plan.numel, dtype=dtype, device=plan.device) for _ in range(2))
+    m, v = (plan.m.new_empty(plan.numel, dtype=dtype) for _ in range(2))
     image, mp, ms, vp, vs, _, _ = plan._fixed
-    check(lib.ppo2hip_adamw_state(plan._tensors, len(plan._ptrs), image, mp, ms, vp, vs, _ADAMW_TYPES[dtype], _ptr(m), _ptr(v),
-                                  _stream()), "adamw_state")
+    check(lib.ppo2hip_adamw_state(plan._tensors, len(plan._ptrs), image, mp, ms, vp, vs, _ADAMW_TYPES[dtype], m.data_ptr(), v.data_ptr(),
+                                  _raw_stream(plan.device.index)), "adamw_state")
     return m, v
 
 
