@@ -3,6 +3,7 @@
 //   g[t] = dy[t] + (reset[t+1] ? 0 : a[t+1] g[t+1])   dx = (1 - a) g   df = g (p - x) a (1 - a)
 // The backward pass recomputes the states from float32 states kept every PPO2HIP_GLR_SPAN steps: they cost
 // 4 / SPAN bytes per element where reading y back costs its whole width, and y is rounded to its type while p - x cancels.
+#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
 
@@ -15,7 +16,6 @@
 namespace ppo2hip {
 
 constexpr int kSpan = PPO2HIP_GLR_SPAN;                     // steps a wave holds in registers at a time
-constexpr int kWaves = 4;                                   // waves of a workgroup that walk
 constexpr int kHeld = 16;                                   // spans that a workgroup can hold at once, one per wave
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -105,19 +105,39 @@ struct Seq {
     int64_t t, e;
 };
 
-// V neighbouring channels of one step, at any address an element may have
+// V neighbouring channels of one step, at any address an element may have.  Inputs of 16 bits stay bits until they are used: as
+// vectors of their type the compiler keeps them in more registers than they have.
 template <class T, int V>
 struct Lane {
-    typedef T Vec __attribute__((ext_vector_type(V)));
-    typedef Vec Any __attribute__((aligned(sizeof(T))));
-    static __device__ inline Vec load(const void *p) { return *(const Any *)p; }
+    typedef T Out __attribute__((ext_vector_type(V)));
+    typedef Out AnyOut __attribute__((aligned(sizeof(T))));
     static __device__ inline void store(void *p, const float (&v)[V]) {
-        Vec r;
+        Out r;
 #pragma unroll
         for (int k = 0; k < V; k++) r[k] = (T)v[k];       // to nearest: the type that the layer hands on; states stay float32
-        *(Any *)p = r;
+        *(AnyOut *)p = r;
     }
 };
+template <int Bytes>
+struct Bits;
+template <>
+struct Bits<2> {
+    typedef unsigned short Word;
+    typedef Word Any __attribute__((aligned(2)));
+};
+template <>
+struct Bits<4> {
+    typedef unsigned Word;
+    typedef Word Any __attribute__((aligned(2)));
+};
+template <class T>
+__device__ inline float widen(unsigned bits);
+template <>
+__device__ inline float widen<float>(unsigned bits) { return __uint_as_float(bits); }
+template <>
+__device__ inline float widen<__bf16>(unsigned bits) { return __uint_as_float(bits << 16); }
+template <>
+__device__ inline float widen<_Float16>(unsigned bits) { return (float)__builtin_bit_cast(_Float16, (unsigned short)bits); }
 
 // Which columns a wave works on.  Addresses are a wave-uniform 64-bit part (step, the wave's first env) and a 32-bit part
 // per lane: kept as 64 bits per lane and step they cost 2 registers each and the kernels spill.
@@ -128,11 +148,11 @@ struct Place {
 };
 // env_tiles 0: columns in a row over all envs.  Else that many tiles per env, where envs lie too far apart for 32 bits.
 template <int V>
-__device__ inline Place place_of(unsigned C, unsigned H, unsigned env_tiles) {
+__device__ inline Place place_of(unsigned tile, unsigned C, unsigned H, unsigned env_tiles) {
     const unsigned lane = threadIdx.x & 63;
     Place p;
     if (env_tiles == 0) {
-        const uint64_t c = ((uint64_t)blockIdx.x * 64 + lane) * V;
+        const uint64_t c = ((uint64_t)tile * 64 + lane) * V;
         p.mine = c < C;
         p.c = p.mine ? (unsigned)c : C - V;
         const unsigned e = p.c / H;
@@ -140,7 +160,7 @@ __device__ inline Place place_of(unsigned C, unsigned H, unsigned env_tiles) {
         p.de = (int)e - p.e0;
         p.j = (int)(p.c - e * H);
     } else {
-        const unsigned e = blockIdx.x / env_tiles, j = ((blockIdx.x - e * env_tiles) * 64 + lane) * V;
+        const unsigned e = tile / env_tiles, j = ((tile - e * env_tiles) * 64 + lane) * V;
         p.mine = j < H;
         p.j = (int)(p.mine ? j : H - V);
         p.e0 = (int)e;
@@ -152,6 +172,12 @@ __device__ inline Place place_of(unsigned C, unsigned H, unsigned env_tiles) {
 template <class T>
 __device__ inline unsigned lane_offset(const Seq<T> &s, const Place &at) {
     return (unsigned)(at.de * (int)s.e + at.j) * (unsigned)sizeof(T);
+}
+// A lane's offset, said anew where it is used: extended to 64 bits in another block it is no longer seen to be 32, and every
+// access adds 64-bit addresses in vector registers instead of taking a scalar base and this.
+__device__ inline unsigned here(unsigned off) {
+    asm volatile("" : "+v"(off));
+    return off;
 }
 // A step's distance in bytes, said anew for every span: as loop invariants the 16 multiples of every array's distance are kept
 // in scalar registers, which do not hold them.
@@ -185,18 +211,25 @@ __device__ inline unsigned span_resets(const Seq<const uint8_t> &r, int64_t t0, 
 
 template <class T, int V>
 struct Raw {
-    typename Lane<T, V>::Vec v[kSpan];
+    typedef Bits<sizeof(T) * V> Kind;
+    typename Kind::Word v[kSpan];
+    __device__ inline float get(int i, int k) const {
+        if (sizeof(T) == 4 || V == 1) return widen<T>(v[i]);
+        return widen<T>(k == 0 ? v[i] & 0xffffu : (unsigned)v[i] >> 16);
+    }
+    static __device__ inline typename Kind::Word one(const char *p) { return *(const typename Kind::Any *)p; }
     __device__ inline void load(const Seq<const T> &s, const Place &at, unsigned off, int64_t t0, int n) {
         const char *p = step_base(s, at, t0);
         const int64_t step = distance(s);
         if (n >= kSpan) {
+            off = here(off);
 #pragma unroll
-            for (int i = 0; i < kSpan; i++, p += step) v[i] = Lane<T, V>::load(p + off);
+            for (int i = 0; i < kSpan; i++, p += step) v[i] = one(p + off);
         } else {
 #pragma unroll
             for (int i = 0; i < kSpan; i++, p += step) {
-                v[i] = (typename Lane<T, V>::Vec)(T)0.f;
-                if (i < n) v[i] = Lane<T, V>::load(p + off);
+                v[i] = 0;
+                if (i < n) v[i] = one(p + off);
             }
         }
     }
@@ -209,17 +242,27 @@ struct Raw {
 template <int V>
 using Span = float[kSpan][V];
 
-// A span's gates and what each step adds to the state, u = (1 - a) x.  Steps behind the last one keep the state as it is;
-// a step with a reset has its gate shut once u is formed, which multiplies a finite state by zero.
-template <class T, int V, bool BACK = false>
-__device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, unsigned rm, Span<V> &g, Span<V> &u) {
+// The value, of which the compiler knows nothing: what the seldom walked slow paths derive from a span is otherwise worked out,
+// and kept in registers, ahead of the branch to them.
+__device__ inline float anew(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+__device__ inline unsigned anew(unsigned v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// A span's gates and what each step adds to the state, u = (1 - a) x.  Steps behind the last one keep the state as it is.
+template <class T, int V>
+__device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, Span<V> &g, Span<V> &u) {
     typedef Gate<sizeof(T) == 4> G;
 #pragma unroll
     for (int i = 0; i < kSpan; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            g[i][k] = G::of((float)f.v[i][k] + b[k]);
-            u[i][k] = BACK ? (float)x.v[i][k] : G::take(g[i][k]) * (float)x.v[i][k];
+            g[i][k] = G::of(f.get(i, k) + b[k]);
+            u[i][k] = G::take(g[i][k]) * x.get(i, k);
         }
     if (n < kSpan)
 #pragma unroll
@@ -227,39 +270,41 @@ __device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const f
 #pragma unroll
             for (int k = 0; k < V; k++)
                 if (i >= n) g[i][k] = G::open(), u[i][k] = 0.f;
-    if (__any(rm != 0))
-#pragma unroll
-        for (int i = 0; i < kSpan; i++)
-#pragma unroll
-            for (int k = 0; k < V; k++) g[i][k] = rm >> i & 1 ? G::shut() : g[i][k];
 }
 
-// Walks a span from state h, handing every step's state to `out(i, h)`.  The quick form of a step has no value for an infinite
-// state and turns it to NaN; NaN goes through shut gates, so a span that met either ends in NaN and is walked again the slow way.
-template <bool EXACT, int V, class Out>
-__device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm, float (&h)[V], Out out) {
-    typedef Gate<EXACT> G;
-    float h0[V];
+template <int V>
+__device__ inline bool any_not_finite(const float (&h)[V]) {
     bool bad = false;
 #pragma unroll
-    for (int k = 0; k < V; k++) h0[k] = h[k];
-#pragma unroll
-    for (int i = 0; i < kSpan; i++) {
-#pragma unroll
-        for (int k = 0; k < V; k++) h[k] = G::pass(g[i][k], h[k]) + u[i][k];
-        out(i, h);
-    }
-#pragma unroll
     for (int k = 0; k < V; k++) bad |= !(fabsf(h[k]) < INFINITY);
-    if (__any(bad)) {
+    return __any(bad);
+}
+
+// Walks a span from state h, handing every step's state to `out(i, h)`: the quick way where no lane has a reset and `whole` says
+// that out may be called for all steps, the general way (out only for steps below n) elsewhere.  The quick form of a step turns an
+// infinite state to NaN, which then stays to the span's end: the span is walked again.
+template <bool EXACT, int V, class Out>
+__device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm, bool whole, int n, float (&h)[V], Out out) {
+    typedef Gate<EXACT> G;
+    if (whole && !__any(rm != 0)) {
+        float h0[V];
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = h0[k];
+        for (int k = 0; k < V; k++) h0[k] = h[k];
 #pragma unroll
         for (int i = 0; i < kSpan; i++) {
 #pragma unroll
-            for (int k = 0; k < V; k++) h[k] = rm >> i & 1 ? u[i][k] : G::pass_any(g[i][k], h[k]) + u[i][k];
+            for (int k = 0; k < V; k++) h[k] = G::pass(g[i][k], h[k]) + u[i][k];
             out(i, h);
         }
+        if (!any_not_finite(h)) return;
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = h0[k];
+    }
+#pragma unroll
+    for (int i = 0; i < kSpan; i++) {
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = anew(rm) >> i & 1 ? u[i][k] : G::pass_any(anew(g[i][k]), h[k]) + u[i][k];
+        if (i < n) out(i, h);
     }
 }
 
@@ -282,141 +327,205 @@ __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run (&r)[V]) {
         if (rm) r[k].A = -1.f;
 }
 
-// The same against time, for the gradient: dy enters a step before the gate does, a reset stands behind it.
+// A span's run in the direction of time,
 template <bool EXACT, int V>
-__device__ inline void span_back(const Span<V> &g, const Span<V> &dy, unsigned rm, Run (&r)[V]) {
-    typedef Gate<EXACT> G;
-    bool bad = false;
+__device__ inline void span_run(const Span<V> &g, const Span<V> &u, unsigned rm, Run (&r)[V]) {
+    float h[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) r[k].B = 0.f;
+    for (int k = 0; k < V; k++) h[k] = 0.f;
+    span_passes<EXACT, V>(g, rm, r);
+    span_walk<EXACT, V>(g, u, rm, true, kSpan, h, [](int, const float (&)[V]) {});
 #pragma unroll
-    for (int i = kSpan - 1; i >= 0; i--)
+    for (int k = 0; k < V; k++) r[k].B = h[k];
+}
+// and against it, for the gradient: dy enters a step before the gate does, a reset stands behind it.
+template <class T>
+__device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsigned rm, Run (&r)[1]) {
+    typedef Gate<sizeof(T) == 4> G;
+    span_passes<sizeof(T) == 4, 1>(g, rm, r);
+    float c[1] = {0.f};
+    if (!__any(rm != 0)) {
 #pragma unroll
-        for (int k = 0; k < V; k++) r[k].B = G::pass(g[i][k], r[k].B + dy[i][k]);
-#pragma unroll
-    for (int k = 0; k < V; k++) bad |= !(fabsf(r[k].B) < INFINITY);
-    if (__any(bad)) {
-#pragma unroll
-        for (int k = 0; k < V; k++) r[k].B = 0.f;
-#pragma unroll
-        for (int i = kSpan - 1; i >= 0; i--)
-#pragma unroll
-            for (int k = 0; k < V; k++) r[k].B = rm >> i & 1 ? 0.f : G::pass_any(g[i][k], r[k].B + dy[i][k]);
+        for (int i = kSpan - 1; i >= 0; i--) c[0] = G::pass(g[i][0], c[0] + dy.get(i, 0));
+        r[0].B = c[0];
+        if (!any_not_finite(c)) return;
+        c[0] = 0.f;
     }
+#pragma unroll
+    for (int i = kSpan - 1; i >= 0; i--) c[0] = anew(rm) >> i & 1 ? 0.f : G::pass_any(anew(g[i][0]), c[0] + dy.get(i, 0));
+    r[0].B = c[0];
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// how a sequence is cut
+// a chain of workgroups
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Shares: every wave walks `spans` spans of its tile of columns; kWaves shares in a row make a segment, a workgroup's.  With one
-// share per tile (segs = 1, shares = 1) a wave walks the whole sequence.  Else a first launch finds what every share does to the
-// state that enters it, and the second starts every share from what the shares before it make of h0.
-struct Shares {
-    int spans, shares, segs;
-    float *seg_runs;        // [segs][3][C]
-    float *share_runs;      // [segs * kWaves][3][C]
+// Long sequences of few columns in one pass over the data: a workgroup holds kChainWaves spans of a tile in registers, a batch,
+// and the batches of a tile hand each other what they do to the state.  Workgroups draw batches from one counter, all tiles' first
+// ones before all second ones, so that whatever a batch waits for has been drawn by a workgroup that is running and that itself
+// only waits for earlier ones.  A batch
+// publishes its run; kGroup batches in a row form a group, whose last one publishes the state behind it instead.  A batch waits
+// for the runs of its group's earlier batches and for the state in front of the group: what is joined with what does not depend
+// on who came first, so that results are the same bits every time.
+// A word is published by one agent-scope store and is its own flag: a launch before fills all words with kEmpty, a NaN that no
+// arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with zeros.
+constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan, kGroup = 32;
+constexpr unsigned kEmpty = 0xffffffffu;
+
+struct Chain {
+    unsigned *turn;         // the counter, in 256 bytes of its own; then
+    float *runs;            // [batches][A, D, B][C]
+    float *states;          // [groups][C]: in front of groups 1, 2, ...
+    unsigned tiles;
+    int batches, max_spins;
+    unsigned *fault;
 };
 
-// State that enters share `w` of segment `seg` (BACK: gradient, from the other end).  Every wave joins a part of the segments
-// before it, the parts meet in LDS; then the segment's own shares.
-template <int V, bool BACK>
-__device__ inline void shares_through(const Shares &cut, unsigned C, unsigned c, int seg, int w, float (&part)[kWaves][3][64 * V], float (&h)[V]) {
-    const int lane = threadIdx.x & 63;
-    const int n = BACK ? cut.segs - 1 - seg : seg, per = (n + kWaves - 1) / kWaves;
-    if (n > 0) {
-        const int lo = w * per, hi = lo + per < n ? lo + per : n;
-        Run r[V];
-#pragma unroll
-        for (int k = 0; k < V; k++) r[k] = {1.f, 0.f, 0.f};
-#pragma unroll 8
-        for (int i = lo; i < hi; i++) {
-            const float *q = cut.seg_runs + (int64_t)(BACK ? cut.segs - 1 - i : i) * 3 * C + c;
-#pragma unroll
-            for (int k = 0; k < V; k++) r[k] = run_join(r[k], Run{q[k], q[(int64_t)C + k], q[2 * (int64_t)C + k]});
-        }
-#pragma unroll
-        for (int k = 0; k < V; k++) part[w][0][lane * V + k] = r[k].A, part[w][1][lane * V + k] = r[k].D, part[w][2][lane * V + k] = r[k].B;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWaves; i++)
-#pragma unroll
-            for (int k = 0; k < V; k++) h[k] = run_through(Run{part[i][0][lane * V + k], part[i][1][lane * V + k], part[i][2][lane * V + k]}, h[k]);
-    }
-    for (int i = BACK ? kWaves - 1 : 0; i != w; i += BACK ? -1 : 1) {
-        const float *q = cut.share_runs + ((int64_t)seg * kWaves + i) * 3 * C + c;
-#pragma unroll
-        for (int k = 0; k < V; k++) h[k] = run_through(Run{q[k], q[(int64_t)C + k], q[2 * (int64_t)C + k]}, h[k]);
-    }
+__device__ inline void publish(float *p, float v) {
+    const unsigned bits = __float_as_uint(v);
+    __hip_atomic_store((unsigned *)p, bits == kEmpty ? 0x7fc00000u : bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// from a base that the wave shares
+__device__ inline unsigned peek(const float *base, unsigned c) {
+    return __hip_atomic_load((const unsigned *)((const char *)base + c), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// First launch of a sequence that is cut: the runs of every share and segment.  x stands for dy when BACK.
-template <class T, int V, bool BACK>
-__global__ __launch_bounds__(64 * kWaves) void glr_runs_kernel(Seq<const T> f, Seq<const T> x, const float *__restrict__ bias,
-                                                               Seq<const uint8_t> resets, int T_, unsigned C, unsigned H, unsigned env_tiles,
-                                                               Shares cut) {
-    __shared__ float part[kWaves][3][64 * V];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seg = blockIdx.y;
-    const Place at = place_of<V>(C, H, env_tiles);
-    const unsigned fo = lane_offset(f, at), xo = lane_offset(x, at);
-    float b[V];
-    Run r[V];
+__global__ __launch_bounds__(256) void glr_chain_clear_kernel(Chain ch, int64_t words) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i == 0) *ch.turn = 0;
+    unsigned *p = (unsigned *)ch.runs + i;
+    if (i + 4 <= words) *(uint4 *)p = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
+    else
+        for (int k = 0; i + k < words; k++) p[k] = kEmpty;
+}
+
+template <int V>
+struct ChainSpace {
+    float runs[kChainWaves][3][64 * V], before[kChainWaves][3][64 * V], state[64 * V];
+    unsigned turn;
+};
+
+// State (gradient, when BACK) in front of wave w's span, from the span's own run and the value h in front of the whole sequence.
+// All waves of the workgroup call it; publishes what later batches wait for.
+template <bool BACK, int V>
+__device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned C, const Place &at, int order, int w, const Run (&own)[V],
+                                     float (&h)[V]) {
+    const int lane = (threadIdx.x & 63) * V, group = order / kGroup, rank = order - group * kGroup;
 #pragma unroll
-    for (int k = 0; k < V; k++) b[k] = bias ? bias[at.j + k] : 0.f, r[k] = {1.f, 0.f, 0.f};
-    const int64_t first = ((int64_t)seg * kWaves + w) * cut.spans, last = (T_ + kSpan - 1) / kSpan;
-    const int64_t end = first + cut.spans < last ? first + cut.spans : last;
-    Raw<T, V> fr, xr;
-    auto fetch = [&](int64_t s) {
-        const int64_t t0 = s * kSpan;
-        const int n = (int)(T_ - t0 < kSpan ? T_ - t0 : kSpan);
-        fr.load(f, at, fo, t0, n);
-        xr.load(x, at, xo, t0, n);
-    };
-    if (first < end) fetch(BACK ? end - 1 : first);
-    for (int64_t i = first; i < end; i++) {
-        const int64_t s = BACK ? end - 1 - (i - first) : i, t0 = s * kSpan;
-        const int n = (int)(T_ - t0 < kSpan ? T_ - t0 : kSpan);
-        const unsigned rm = span_resets(resets, t0, n, at);
-        Span<V> g, u;                                       // BACK: u is dy
-        Run one[V];
-        span_open<T, V, BACK>(fr, xr, b, n, rm, g, u);
-        if (i + 1 < end) fetch(BACK ? s - 1 : s + 1);
-        span_passes<sizeof(T) == 4, V>(g, rm, one);
-        if (BACK) {
-            span_back<sizeof(T) == 4, V>(g, u, rm, one);
-        } else {
-            float h[V];
-#pragma unroll
-            for (int k = 0; k < V; k++) h[k] = 0.f;
-            span_walk<sizeof(T) == 4, V>(g, u, rm, h, [](int, const float (&)[V]) {});
-#pragma unroll
-            for (int k = 0; k < V; k++) one[k].B = h[k];
-        }
-#pragma unroll
-        for (int k = 0; k < V; k++) r[k] = run_join(r[k], one[k]);
-    }
-    float *own = cut.share_runs + ((int64_t)seg * kWaves + w) * 3 * C + at.c;
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-        if (at.mine) own[k] = r[k].A, own[(int64_t)C + k] = r[k].D, own[2 * (int64_t)C + k] = r[k].B;
-        part[w][0][lane * V + k] = r[k].A;
-        part[w][1][lane * V + k] = r[k].D;
-        part[w][2][lane * V + k] = r[k].B;
-    }
+    for (int k = 0; k < V; k++) m.runs[w][0][lane + k] = own[k].A, m.runs[w][1][lane + k] = own[k].D, m.runs[w][2][lane + k] = own[k].B;
     __syncthreads();
-    if (w == 0 && at.mine) {
-        float *o = cut.seg_runs + (int64_t)seg * 3 * C + at.c;
+    if (w == kChainWaves - 1 && rank < kGroup - 1 && order + 1 < ch.batches && at.mine) {
 #pragma unroll
         for (int k = 0; k < V; k++) {
             Run all = {1.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < kWaves; i++) {
-                const int q = BACK ? kWaves - 1 - i : i;
-                all = run_join(all, Run{part[q][0][lane * V + k], part[q][1][lane * V + k], part[q][2][lane * V + k]});
+            for (int i = 0; i < kChainWaves; i++) {
+                const int q = BACK ? kChainWaves - 1 - i : i;
+                all = run_join(all, Run{m.runs[q][0][lane + k], m.runs[q][1][lane + k], m.runs[q][2][lane + k]});
             }
-            o[k] = all.A, o[(int64_t)C + k] = all.D, o[2 * (int64_t)C + k] = all.B;
+            float *o = ch.runs + (int64_t)order * 3 * C + at.c + k;
+            publish(o, all.A), publish(o + C, all.D), publish(o + 2 * (int64_t)C, all.B);
         }
     }
+    const unsigned byte = at.c * 4u;                      // a chain has few columns
+    // the group's earlier batches, up to kEach to a wave
+    constexpr int kEach = kGroup / kChainWaves;
+    const int lo = w * kEach;
+    Run r[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) r[k] = {1.f, 0.f, 0.f};
+    if (lo < rank) {
+        unsigned bits[kEach][3][V];
+        for (int tries = 0;; tries++) {
+            bool ok = true;
+#pragma unroll
+            for (int i = 0; i < kEach; i++)
+#pragma unroll
+                for (int q = 0; q < 3; q++)
+#pragma unroll
+                    for (int k = 0; k < V; k++)
+                        bits[i][q][k] = lo + i < rank ? peek(ch.runs + ((int64_t)(group * kGroup + lo + i) * 3 + q) * C + k, byte) : 0u;
+#pragma unroll
+            for (int i = 0; i < kEach; i++)
+#pragma unroll
+                for (int q = 0; q < 3; q++)
+#pragma unroll
+                    for (int k = 0; k < V; k++) ok &= bits[i][q][k] != kEmpty;
+            if (__all(ok)) break;
+            if (tries >= ch.max_spins) {
+                if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
+                break;
+            }
+            __builtin_amdgcn_s_sleep(1);
+        }
+#pragma unroll
+        for (int i = 0; i < kEach; i++)
+            if (lo + i < rank)
+#pragma unroll
+                for (int k = 0; k < V; k++)
+                    r[k] = run_join(r[k], Run{__uint_as_float(bits[i][0][k]), __uint_as_float(bits[i][1][k]), __uint_as_float(bits[i][2][k])});
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++) m.before[w][0][lane + k] = r[k].A, m.before[w][1][lane + k] = r[k].D, m.before[w][2][lane + k] = r[k].B;
+    if (w == 0) {
+        if (group > 0) {
+            unsigned bits[V];
+            for (int tries = 0;; tries++) {
+                bool ok = true;
+#pragma unroll
+                for (int k = 0; k < V; k++) bits[k] = peek(ch.states + (int64_t)group * C + k, byte);
+#pragma unroll
+                for (int k = 0; k < V; k++) ok &= bits[k] != kEmpty;
+                if (__all(ok)) break;
+                if (tries >= ch.max_spins) {
+                    if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
+                    break;
+                }
+                __builtin_amdgcn_s_sleep(1);
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) h[k] = __uint_as_float(bits[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < V; k++) m.state[lane + k] = h[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < V; k++) h[k] = m.state[lane + k];
+    const int waves = (rank + kEach - 1) / kEach;
+    for (int i = 0; i < waves; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = run_through(Run{m.before[i][0][lane + k], m.before[i][1][lane + k], m.before[i][2][lane + k]}, h[k]);
+    const int steps = BACK ? kChainWaves - 1 - w : w;
+    for (int i = 0; i < steps; i++) {
+        const int q = BACK ? kChainWaves - 1 - i : i;
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = run_through(Run{m.runs[q][0][lane + k], m.runs[q][1][lane + k], m.runs[q][2][lane + k]}, h[k]);
+    }
+    // the last batch of a group hands on the state behind it; the last wave in the chain's direction has it
+    if (steps == kChainWaves - 1 && rank == kGroup - 1 && order + 1 < ch.batches && at.mine)
+#pragma unroll
+        for (int k = 0; k < V; k++) publish(ch.states + (int64_t)(group + 1) * C + at.c + k, run_through(own[k], h[k]));
+}
+
+// The batch that this workgroup draws: its tile's columns and wave w's span in it.
+struct Drawn {
+    Place at;
+    int order, batch, n;
+    int64_t t0;
+};
+template <bool BACK, int V, class Args>
+__device__ inline Drawn draw(const Args &a, const Chain &ch, unsigned &turn, int w) {
+    if (threadIdx.x == 0) turn = atomicAdd(ch.turn, 1u);
+    __syncthreads();
+    const unsigned u = __builtin_amdgcn_readfirstlane(turn);
+    Drawn d;
+    d.order = (int)(u / ch.tiles);
+    d.batch = BACK ? ch.batches - 1 - d.order : d.order;
+    d.at = place_of<V>(u - (unsigned)d.order * ch.tiles, a.C, a.H, a.env_tiles);
+    d.t0 = ((int64_t)d.batch * kChainWaves + w) * kSpan;
+    d.n = (int)(a.T_ - d.t0 < kSpan ? a.T_ - d.t0 : kSpan);
+    return d;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -437,37 +546,28 @@ struct ForwardArgs {
 template <class T, int V>
 __device__ inline void forward_span(const ForwardArgs<T> &a, const Place &at, unsigned yo, int64_t t0, int n, unsigned rm, const Span<V> &g,
                                     const Span<V> &u, float (&h)[V]) {
-    if (a.saved && at.mine)
+    if (!at.mine) return;
+    if (a.saved)
 #pragma unroll
         for (int k = 0; k < V; k++) a.saved[t0 / kSpan * a.C + at.c + k] = h[k];
-    char *base = step_base(a.y, at, t0);
+    char *p = nullptr;
     const int64_t step = distance(a.y);
-    span_walk<sizeof(T) == 4, V>(g, u, rm, h, [&](int i, const float (&v)[V]) {
-        if (i < n && at.mine) Lane<T, V>::store(base + i * step + yo, v);
+    span_walk<sizeof(T) == 4, V>(g, u, rm, n >= kSpan, n, h, [&](int i, const float (&v)[V]) {
+        p = i == 0 ? step_base(a.y, at, t0) : p + step;
+        Lane<T, V>::store(p + here(yo), v);
     });
-    if (a.h_last && t0 + kSpan >= a.T_ && at.mine)
+    if (a.h_last && t0 + kSpan >= a.T_)
 #pragma unroll
         for (int k = 0; k < V; k++) a.h_last[at.c + k] = h[k];
 }
 
-// Every wave walks its share; the next span's inputs are on their way while a span is walked.
+// A wave walks spans first .. end-1 of its columns from state h; the next span's inputs are on their way while a span is walked.
 template <class T, int V>
-__global__ __launch_bounds__(64 * kWaves) void glr_forward_kernel(ForwardArgs<T> a, Shares cut) {
-    __shared__ float part[kWaves][3][64 * V];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seg = cut.shares == 1 ? 0 : (int)(gridDim.y - 1 - blockIdx.y);
-    const Place at = place_of<V>(a.C, a.H, a.env_tiles);
+__device__ inline void forward_walk(const ForwardArgs<T> &a, const Place &at, int64_t first, int64_t end, float (&h)[V]) {
     const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at), yo = lane_offset(a.y, at);
-    float b[V], h[V];
+    float b[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f, h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
-    int64_t span = 0, end = cut.spans;
-    if (cut.shares > 1) {
-        shares_through<V, false>(cut, a.C, at.c, seg, w, part, h);
-        span = ((int64_t)seg * kWaves + w) * cut.spans;
-        end = span + cut.spans;
-    }
-    const int64_t last = (a.T_ + kSpan - 1) / kSpan;
-    if (end > last) end = last;
+    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f;
     Raw<T, V> fr, xr;
     auto fetch = [&](int64_t s) {
         const int64_t t0 = s * kSpan;
@@ -475,16 +575,26 @@ __global__ __launch_bounds__(64 * kWaves) void glr_forward_kernel(ForwardArgs<T>
         fr.load(a.f, at, fo, t0, n);
         xr.load(a.x, at, xo, t0, n);
     };
-    if (span < end) fetch(span);
-    for (; span < end; span++) {
+    if (first < end) fetch(first);
+    for (int64_t span = first; span < end; span++) {
         const int64_t t0 = span * kSpan;
         const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
         const unsigned rm = span_resets(a.resets, t0, n, at);
         Span<V> g, u;
-        span_open<T, V>(fr, xr, b, n, rm, g, u);
+        span_open<T, V>(fr, xr, b, n, g, u);
         if (span + 1 < end) fetch(span + 1);
         forward_span<T, V>(a, at, yo, t0, n, rm, g, u, h);
     }
+}
+
+// One wave per tile.
+template <class T, int V>
+__global__ __launch_bounds__(64) void glr_forward_kernel(ForwardArgs<T> a) {
+    const Place at = place_of<V>(blockIdx.x, a.C, a.H, a.env_tiles);
+    float h[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
+    forward_walk<T, V>(a, at, 0, (a.T_ + kSpan - 1) / kSpan, h);
 }
 
 // Short sequences of few columns in one launch: a workgroup holds the whole of its columns, one span per wave, and the waves
@@ -493,7 +603,7 @@ template <class T, int V>
 __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArgs<T> a) {
     __shared__ float runs[kHeld][3][64 * V];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Place at = place_of<V>(a.C, a.H, a.env_tiles);
+    const Place at = place_of<V>(blockIdx.x, a.C, a.H, a.env_tiles);
     const int64_t t0 = (int64_t)w * kSpan;
     const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
     Raw<T, V> fr, xr;
@@ -502,15 +612,14 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
     const unsigned rm = span_resets(a.resets, t0, n, at);
     float b[V], h[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f, h[k] = 0.f;
+    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f;
     Span<V> g, u;
     Run r[V];
-    span_open<T, V>(fr, xr, b, n, rm, g, u);
-    span_passes<sizeof(T) == 4, V>(g, rm, r);
-    span_walk<sizeof(T) == 4, V>(g, u, rm, h, [](int, const float (&)[V]) {});
+    span_open<T, V>(fr, xr, b, n, g, u);
+    span_run<sizeof(T) == 4, V>(g, u, rm, r);
 #pragma unroll
     for (int k = 0; k < V; k++) {
-        runs[w][0][lane * V + k] = r[k].A, runs[w][1][lane * V + k] = r[k].D, runs[w][2][lane * V + k] = h[k];
+        runs[w][0][lane * V + k] = r[k].A, runs[w][1][lane * V + k] = r[k].D, runs[w][2][lane * V + k] = r[k].B;
         h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
     }
     __syncthreads();
@@ -518,6 +627,28 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
 #pragma unroll
         for (int k = 0; k < V; k++) h[k] = run_through(Run{runs[i][0][lane * V + k], runs[i][1][lane * V + k], runs[i][2][lane * V + k]}, h[k]);
     forward_span<T, V>(a, at, lane_offset(a.y, at), t0, n, rm, g, u, h);
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_chain_kernel(ForwardArgs<T> a, Chain ch) {
+    __shared__ ChainSpace<V> mem;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Drawn d = draw<false, V>(a, ch, mem.turn, w);
+    Raw<T, V> fr, xr;
+    fr.load(a.f, d.at, lane_offset(a.f, d.at), d.t0, d.n);
+    xr.load(a.x, d.at, lane_offset(a.x, d.at), d.t0, d.n);
+    const unsigned rm = span_resets(a.resets, d.t0, d.n, d.at);
+    float b[V], h[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[d.at.j + k] : 0.f;
+    Span<V> g, u;
+    Run r[V];
+    span_open<T, V>(fr, xr, b, d.n, g, u);
+    span_run<sizeof(T) == 4, V>(g, u, rm, r);
+#pragma unroll
+    for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[d.at.c + k] : 0.f;
+    chain_through<false, V>(ch, mem, a.C, d.at, d.order, w, r, h);
+    if (d.n > 0) forward_span<T, V>(a, d.at, lane_offset(a.y, d.at), d.t0, d.n, rm, g, u, h);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -530,145 +661,116 @@ struct BackwardArgs {
     Seq<const uint8_t> resets;
     Seq<T> df, dx;
     const float *bias, *saved, *dh_last;
-    float *dbias_rows, *dh0;        // dbias_rows [segs][C] or null
+    float *dbias_rows, *dh0;        // dbias_rows [workgroups along time][C] or null
     int T_;
     unsigned C, H, env_tiles;
 };
 
-// Gates (resets not in them) and q = (p - x) a (1 - a), what df is per unit of g, from the states recomputed off the kept one.
-template <class T, int V>
-__device__ inline void back_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], const float (&kept)[V], int n, unsigned rm,
-                                 Span<V> &g, Span<V> &q) {
+// Gates and q = (p - x) a (1 - a), what df is per unit of g, from the states recomputed off the kept one.
+template <class T>
+__device__ inline void back_open(const Raw<T, 1> &f, const Raw<T, 1> &x, float b, float kept, int n, unsigned rm, Span<1> &g, Span<1> &q) {
     typedef Gate<sizeof(T) == 4> G;
-    float h[V];
-    bool bad = false;
+    float h[1] = {kept}, slope;
+    bool done = false;
+    if (!__any(rm != 0)) {
 #pragma unroll
-    for (int k = 0; k < V; k++) h[k] = kept[k];
-#pragma unroll
-    for (int i = 0; i < kSpan; i++)
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            float slope;
-            const float xv = (float)x.v[i][k];
-            g[i][k] = G::of((float)f.v[i][k] + b[k], slope);
-            if (rm >> i & 1) h[k] = 0.f;
-            q[i][k] = (h[k] - xv) * slope;
-            bad |= !(fabsf(h[k]) < INFINITY);
-            h[k] = G::pass(g[i][k], h[k]) + G::take(g[i][k]) * xv;
+        for (int i = 0; i < kSpan; i++) {
+            const float xv = x.get(i, 0), v = G::of(f.get(i, 0) + b, slope);
+            g[i][0] = v;
+            q[i][0] = (h[0] - xv) * slope;
+            h[0] = G::pass(v, h[0]) + G::take(v) * xv;
         }
-    if (__any(bad)) {
+        done = !any_not_finite(h);
+    }
+    if (!done) {
+        h[0] = kept;
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = kept[k];
-#pragma unroll
-        for (int i = 0; i < kSpan; i++)
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                float slope;
-                const float xv = (float)x.v[i][k];
-                g[i][k] = G::of((float)f.v[i][k] + b[k], slope);
-                if (rm >> i & 1) h[k] = 0.f;
-                q[i][k] = (h[k] - xv) * slope;
-                h[k] = G::pass_any(g[i][k], h[k]) + G::take(g[i][k]) * xv;
-            }
+        for (int i = 0; i < kSpan; i++) {
+            const float xv = anew(x.get(i, 0)), v = G::of(anew(f.get(i, 0)) + b, slope);
+            if (anew(rm) >> i & 1) h[0] = 0.f;
+            g[i][0] = v;
+            q[i][0] = (h[0] - xv) * slope;
+            h[0] = G::pass_any(v, h[0]) + G::take(v) * xv;
+        }
     }
     if (n < kSpan)
 #pragma unroll
         for (int i = 0; i < kSpan; i++)
-#pragma unroll
-            for (int k = 0; k < V; k++)
-                if (i >= n) g[i][k] = G::open(), q[i][k] = 0.f;
+            if (i >= n) g[i][0] = G::open(), q[i][0] = 0.f;
 }
 
 // Walks a span back from gradient `in`, writes df and dx and adds up df.
-template <class T, int V>
+template <class T>
 __device__ inline void back_span(const BackwardArgs<T> &a, const Place &at, unsigned dfo, unsigned dxo, int64_t t0, int n, unsigned rm,
-                                 const Span<V> &g, const Span<V> &q, const Raw<T, V> &dy, float (&in)[V], double (&total)[V]) {
+                                 const Span<1> &g, const Span<1> &q, const Raw<T, 1> &dy, float &in, double &total) {
     typedef Gate<sizeof(T) == 4> G;
-    char *fp = step_base(a.df, at, t0), *xp = step_base(a.dx, at, t0);
+    if (!at.mine) return;
+    char *fp = nullptr, *xp = nullptr;
     const int64_t fstep = distance(a.df), xstep = distance(a.dx);
-    float sum[V], in0[V];
-    bool bad = false;
-    auto walk = [&](auto slow) {
-#pragma unroll
-        for (int k = 0; k < V; k++) sum[k] = 0.f;
-#pragma unroll
-        for (int i = kSpan - 1; i >= 0; i--) {
-            float of[V], ox[V];
-#pragma unroll
-            for (int k = 0; k < V; k++) {
-                const float gs = (float)dy.v[i][k] + in[k];
-                ox[k] = G::take(g[i][k]) * gs;
-                of[k] = gs * q[i][k];
-                sum[k] += of[k];
-                in[k] = decltype(slow)::value ? G::pass_any(g[i][k], gs) : G::pass(g[i][k], gs);
-                bad |= !(fabsf(in[k]) < INFINITY);
-                if (rm >> i & 1) in[k] = 0.f;
-            }
-            if (i < n && at.mine) {
-                Lane<T, V>::store(fp + i * fstep + dfo, of);
-                Lane<T, V>::store(xp + i * xstep + dxo, ox);
-            }
+    auto put = [&](int i, float of, float ox) {
+        fp = i == kSpan - 1 ? step_base(a.df, at, t0 + kSpan - 1) : fp - fstep;
+        xp = i == kSpan - 1 ? step_base(a.dx, at, t0 + kSpan - 1) : xp - xstep;
+        const float f1[1] = {of}, x1[1] = {ox};
+        if (i < n) {
+            Lane<T, 1>::store(fp + here(dfo), f1);
+            Lane<T, 1>::store(xp + here(dxo), x1);
         }
     };
+    float sum = 0.f, c[1] = {in};
+    bool done = false;
+    if (n >= kSpan && !__any(rm != 0)) {
+        n = kSpan;
 #pragma unroll
-    for (int k = 0; k < V; k++) in0[k] = in[k];
-    walk(std::false_type{});
-    if (__any(bad)) {
-#pragma unroll
-        for (int k = 0; k < V; k++) in[k] = in0[k];
-        walk(std::true_type{});
-    }
-#pragma unroll
-    for (int k = 0; k < V; k++) total[k] += (double)sum[k];
-    if (a.dh0 && t0 == 0 && at.mine)
-#pragma unroll
-        for (int k = 0; k < V; k++) a.dh0[at.c + k] = in[k];
-}
-
-// per segment and column: the waves' sums in wave order
-template <int W, int V>
-__device__ inline void dbias_row(float *row, unsigned c, bool mine, int nw, const double (&total)[V], double (&sums)[W][64 * V]) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-#pragma unroll
-    for (int k = 0; k < V; k++) sums[w][lane * V + k] = total[k];
-    __syncthreads();
-    if (w == 0 && mine)
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-            double s = 0.0;
-            for (int i = 0; i < nw; i++) s += sums[i][lane * V + k];
-            row[c + k] = (float)s;
+        for (int i = kSpan - 1; i >= 0; i--) {
+            const float gs = dy.get(i, 0) + c[0], of = gs * q[i][0];
+            sum += of;
+            put(i, of, G::take(g[i][0]) * gs);
+            c[0] = G::pass(g[i][0], gs);
         }
+        done = !any_not_finite(c);
+    }
+    if (!done) {
+        sum = 0.f;
+        c[0] = in;
+#pragma unroll
+        for (int i = kSpan - 1; i >= 0; i--) {
+            const float v = anew(g[i][0]), gs = dy.get(i, 0) + c[0], of = gs * q[i][0];
+            if (i < n) sum += of;
+            put(i, of, G::take(v) * gs);
+            c[0] = anew(rm) >> i & 1 ? 0.f : G::pass_any(v, gs);
+        }
+    }
+    in = c[0];
+    total += (double)sum;
+    if (a.dh0 && t0 == 0) a.dh0[at.c] = in;
 }
 
-template <class T, int V>
-__global__ __launch_bounds__(64 * kWaves, 2) void glr_backward_kernel(BackwardArgs<T> a, Shares cut) {
-    __shared__ float part[kWaves][3][64 * V];
-    __shared__ double sums[kWaves][64 * V];
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), seg = blockIdx.y;
-    const Place at = place_of<V>(a.C, a.H, a.env_tiles);
-    const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at), go = lane_offset(a.dy, at), dfo = lane_offset(a.df, at), dxo = lane_offset(a.dx, at);
-    float b[V], in[V];
-    double total[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f, in[k] = a.dh_last ? a.dh_last[at.c + k] : 0.f, total[k] = 0.0;
-    int64_t first = 0, end = cut.spans;
-    if (cut.shares > 1) {
-        shares_through<V, true>(cut, a.C, at.c, seg, w, part, in);
-        first = ((int64_t)seg * kWaves + w) * cut.spans;
-        end = first + cut.spans;
+// a workgroup's sums of df per column, the waves' in wave order
+template <int W>
+__device__ inline void dbias_row(float *row, const Place &at, int nw, double total, double (&sums)[W][64]) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    sums[w][lane] = total;
+    __syncthreads();
+    if (w == 0 && at.mine) {
+        double s = 0.0;
+        for (int i = 0; i < nw; i++) s += sums[i][lane];
+        row[at.c] = (float)s;
     }
-    const int64_t last = (a.T_ + kSpan - 1) / kSpan;
-    if (end > last) end = last;
-    Raw<T, V> fr, xr, gr;
-    float kept[V];
+}
+
+// A wave walks spans end-1 .. first of its columns back from gradient `in` and adds up df.
+template <class T>
+__device__ inline void backward_walk(const BackwardArgs<T> &a, const Place &at, int64_t first, int64_t end, float (&in)[1], double (&total)[1]) {
+    const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at), go = lane_offset(a.dy, at), dfo = lane_offset(a.df, at), dxo = lane_offset(a.dx, at);
+    const float b = a.bias ? a.bias[at.j] : 0.f;
+    Raw<T, 1> fr, xr, gr;
+    float kept;
     auto fetch = [&](int64_t s) {
         const int64_t t0 = s * kSpan;
         const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
         fr.load(a.f, at, fo, t0, n);
         xr.load(a.x, at, xo, t0, n);
-#pragma unroll
-        for (int k = 0; k < V; k++) kept[k] = a.saved[s * a.C + at.c + k];
+        kept = a.saved[s * a.C + at.c];
     };
     if (first < end) fetch(end - 1);
     for (int64_t s = end - 1; s >= first; s--) {
@@ -676,56 +778,70 @@ __global__ __launch_bounds__(64 * kWaves, 2) void glr_backward_kernel(BackwardAr
         const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
         gr.load(a.dy, at, go, t0, n);
         const unsigned rm = span_resets(a.resets, t0, n, at);
-        Span<V> g, q;
-        back_open<T, V>(fr, xr, b, kept, n, rm, g, q);
+        Span<1> g, q;
+        back_open<T>(fr, xr, b, kept, n, rm, g, q);
         if (s > first) fetch(s - 1);
-        back_span<T, V>(a, at, dfo, dxo, t0, n, rm, g, q, gr, in, total);
+        back_span<T>(a, at, dfo, dxo, t0, n, rm, g, q, gr, in[0], total[0]);
     }
-    if (a.dbias_rows) dbias_row<kWaves, V>(a.dbias_rows + (int64_t)seg * a.C, at.c, at.mine, cut.shares > 1 ? kWaves : 1, total, sums);
 }
 
-template <class T, int V>
+template <class T>
+__global__ __launch_bounds__(64, 2) void glr_backward_kernel(BackwardArgs<T> a) {
+    const Place at = place_of<1>(blockIdx.x, a.C, a.H, a.env_tiles);
+    float in[1] = {a.dh_last ? a.dh_last[at.c] : 0.f};
+    double total[1] = {0.0};
+    backward_walk<T>(a, at, 0, (a.T_ + kSpan - 1) / kSpan, in, total);
+    if (a.dbias_rows && at.mine) a.dbias_rows[at.c] = (float)total[0];
+}
+
+template <class T>
 __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardArgs<T> a) {
-    __shared__ float runs[kHeld][3][64 * V];
-    __shared__ double sums[kHeld][64 * V];
+    __shared__ float runs[kHeld][3][64];
+    __shared__ double sums[kHeld][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
-    const Place at = place_of<V>(a.C, a.H, a.env_tiles);
+    const Place at = place_of<1>(blockIdx.x, a.C, a.H, a.env_tiles);
     const int64_t t0 = (int64_t)w * kSpan;
     const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
-    Raw<T, V> fr, xr, gr;
+    Raw<T, 1> fr, xr, gr;
     fr.load(a.f, at, lane_offset(a.f, at), t0, n);
     xr.load(a.x, at, lane_offset(a.x, at), t0, n);
     gr.load(a.dy, at, lane_offset(a.dy, at), t0, n);
     const unsigned rm = span_resets(a.resets, t0, n, at);
-    float b[V], kept[V], in[V];
-    double total[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) {
-        b[k] = a.bias ? a.bias[at.j + k] : 0.f;
-        kept[k] = a.saved[(int64_t)w * a.C + at.c + k];
-        in[k] = a.dh_last ? a.dh_last[at.c + k] : 0.f;
-        total[k] = 0.0;
-    }
-    Span<V> g, q;
-    Run r[V];
-    back_open<T, V>(fr, xr, b, kept, n, rm, g, q);
-    span_passes<sizeof(T) == 4, V>(g, rm, r);
-    {
-        Span<V> shut, dy;
-#pragma unroll
-        for (int i = 0; i < kSpan; i++)
-#pragma unroll
-            for (int k = 0; k < V; k++) shut[i][k] = rm >> i & 1 ? Gate<sizeof(T) == 4>::shut() : g[i][k], dy[i][k] = (float)gr.v[i][k];
-        span_back<sizeof(T) == 4, V>(shut, dy, rm, r);
-    }
-#pragma unroll
-    for (int k = 0; k < V; k++) runs[w][0][lane * V + k] = r[k].A, runs[w][1][lane * V + k] = r[k].D, runs[w][2][lane * V + k] = r[k].B;
+    const float b = a.bias ? a.bias[at.j] : 0.f, kept = a.saved[(int64_t)w * a.C + at.c];
+    float in[1] = {a.dh_last ? a.dh_last[at.c] : 0.f};
+    double total[1] = {0.0};
+    Span<1> g, q;
+    Run r[1];
+    back_open<T>(fr, xr, b, kept, n, rm, g, q);
+    span_run_back<T>(g, gr, rm, r);
+    runs[w][0][lane] = r[0].A, runs[w][1][lane] = r[0].D, runs[w][2][lane] = r[0].B;
     __syncthreads();
-    for (int i = nw - 1; i > w; i--)
-#pragma unroll
-        for (int k = 0; k < V; k++) in[k] = run_through(Run{runs[i][0][lane * V + k], runs[i][1][lane * V + k], runs[i][2][lane * V + k]}, in[k]);
-    back_span<T, V>(a, at, lane_offset(a.df, at), lane_offset(a.dx, at), t0, n, rm, g, q, gr, in, total);
-    if (a.dbias_rows) dbias_row<kHeld, V>(a.dbias_rows, at.c, at.mine, nw, total, sums);
+    for (int i = nw - 1; i > w; i--) in[0] = run_through(Run{runs[i][0][lane], runs[i][1][lane], runs[i][2][lane]}, in[0]);
+    back_span<T>(a, at, lane_offset(a.df, at), lane_offset(a.dx, at), t0, n, rm, g, q, gr, in[0], total[0]);
+    if (a.dbias_rows) dbias_row<kHeld>(a.dbias_rows, at, nw, total[0], sums);
+}
+
+template <class T>
+__global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel(BackwardArgs<T> a, Chain ch) {
+    __shared__ ChainSpace<1> mem;
+    __shared__ double sums[kChainWaves][64];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Drawn d = draw<true, 1>(a, ch, mem.turn, w);
+    Raw<T, 1> fr, xr, gr;
+    fr.load(a.f, d.at, lane_offset(a.f, d.at), d.t0, d.n);
+    xr.load(a.x, d.at, lane_offset(a.x, d.at), d.t0, d.n);
+    gr.load(a.dy, d.at, lane_offset(a.dy, d.at), d.t0, d.n);
+    const unsigned rm = span_resets(a.resets, d.t0, d.n, d.at);
+    const float b = a.bias ? a.bias[d.at.j] : 0.f, kept = d.n > 0 ? a.saved[d.t0 / kSpan * a.C + d.at.c] : 0.f;
+    float in[1] = {a.dh_last ? a.dh_last[d.at.c] : 0.f};
+    double total[1] = {0.0};
+    Span<1> g, q;
+    Run r[1];
+    back_open<T>(fr, xr, b, kept, d.n, rm, g, q);
+    span_run_back<T>(g, gr, rm, r);
+    chain_through<true, 1>(ch, mem, a.C, d.at, d.order, w, r, in);
+    if (d.n > 0) back_span<T>(a, d.at, lane_offset(a.df, d.at), lane_offset(a.dx, d.at), d.t0, d.n, rm, g, q, gr, in[0], total[0]);
+    if (a.dbias_rows) dbias_row<kChainWaves>(a.dbias_rows + (int64_t)d.batch * a.C, d.at, kChainWaves, total[0], sums);
 }
 
 // One step: every thread V channels, nothing to share.
@@ -736,7 +852,9 @@ __global__ __launch_bounds__(256) void glr_step_kernel(Seq<const T> f, Seq<const
     const uint64_t at = ((uint64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (at >= C) return;
     const unsigned c = (unsigned)at, e = c / H, j = c - e * H;
-    const auto fr = Lane<T, V>::load(f.p + (int64_t)e * f.e + j), xr = Lane<T, V>::load(x.p + (int64_t)e * x.e + j);
+    typedef Raw<T, V> In;
+    In in;
+    in.v[0] = In::one((const char *)(f.p + (int64_t)e * f.e + j)), in.v[1] = In::one((const char *)(x.p + (int64_t)e * x.e + j));
     const bool fresh = resets.p && resets.p[(int64_t)e * resets.e];
     float h[V];
 #pragma unroll
@@ -744,8 +862,8 @@ __global__ __launch_bounds__(256) void glr_step_kernel(Seq<const T> f, Seq<const
         h[k] = h0 ? h0[c + k] : 0.f;
         if (saved) saved[c + k] = h[k];
         if (fresh) h[k] = 0.f;
-        const float g = G::of((float)fr[k] + (bias ? bias[j + k] : 0.f));
-        h[k] = G::pass_any(g, h[k]) + G::take(g) * (float)xr[k];
+        const float g = G::of(in.get(0, k) + (bias ? bias[j + k] : 0.f));
+        h[k] = G::pass_any(g, h[k]) + G::take(g) * in.get(1, k);
     }
     Lane<T, V>::store(y.p + (int64_t)e * y.e + j, h);
     if (h_last)
@@ -782,8 +900,7 @@ __global__ void glr_copy_state_kernel(const float *src, float *dst, int64_t n) {
 
 using namespace ppo2hip;
 
-constexpr int64_t kWaveTarget = 4096;     // waves that walk shares
-constexpr int64_t kAlone = 640;           // tiles from which a wave walks a whole sequence
+constexpr int64_t kWalkTiles = 896;       // tiles of a 16-bit sequence from which a wave walks all of its columns' steps
 
 template <class T>
 static Seq<T> seq_of(const ppo2hip_seq *s) {
@@ -815,81 +932,75 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
 }
 
 // How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile, walked by
-// one wave per tile, or cut into shares.
+// one wave per tile, or passed along a chain of workgroups.  Measured, us forward / backward:
+//   [128, E, H] float32, 1024 tiles: held 18.5 / 29.2, walked 21.6 / 35.4; 4096 tiles: 83 / 138, 86 / 138
+//   [2048, E, H] float32, 384 tiles: chain 125 / 197, walked 226 / 491; 2048 tiles: 624 / 1056, 688 / 1127
+//   [512, E, H] bfloat16, 768 tiles: chain 75 / 140, walked 72 / 139; 1024: 97 / 185, 87 / 152; 4096: 365 / 718, 347 / 583
 struct Cut {
-    int V, run_V, env_tiles, run_env_tiles;     // run_*: of the launch that finds the shares' runs
-    int64_t tiles, run_tiles;
-    bool held;
-    Shares sh;
+    enum { kHold, kWalk, kChain } how;
+    int V, env_tiles, batches;
+    int64_t tiles;
 };
 static Cut cut_of(int dtype, int T, int E, int H, bool back) {
     Cut k;
-    const int64_t C = (int64_t)E * H, spans = ceil_div(T, kSpan);
+    const int64_t C = (int64_t)E * H;
     const int wide = dtype != PPO2HIP_F32 && H % 2 == 0 ? 2 : 1;
-    k.env_tiles = k.run_env_tiles = 0;
-    k.run_V = wide;
-    k.run_tiles = ceil_div(C, 64 * wide);
-    k.held = spans <= kHeld && k.run_tiles < kAlone;
-    // two channels per lane halve a 16-bit sequence's loads; the backward walk and the held spans have no registers for them
-    k.V = back || k.held ? 1 : wide;
+    k.how = T <= kHeld * kSpan ? Cut::kHold : dtype != PPO2HIP_F32 && ceil_div(C, 64 * wide) >= kWalkTiles ? Cut::kWalk : Cut::kChain;
+    // two channels per lane halve a 16-bit sequence's loads and double what is in flight; going back there are no registers for them
+    k.V = back ? 1 : wide;
     k.tiles = ceil_div(C, 64 * k.V);
-    k.sh = Shares{(int)spans, 1, 1, nullptr, nullptr};
-    if (k.held || k.run_tiles >= kAlone) return k;
-    int64_t want = ceil_div(kWaveTarget, k.run_tiles);
-    if (want > spans) want = spans;
-    k.sh.spans = (int)ceil_div(spans, want);
-    k.sh.segs = (int)ceil_div(spans, (int64_t)k.sh.spans * kWaves);
-    k.sh.shares = k.sh.segs * kWaves;
+    k.env_tiles = 0;
+    k.batches = k.how == Cut::kChain ? (int)ceil_div(T, kBatch) : 1;
     return k;
 }
 // Lanes of a tile in a row reach over up to 64 V / H envs behind the first: their offsets must fit 31 bits in every array,
 // else each env gets tiles of its own (lanes behind H idle there).
 static void place_envs(Cut &k, int E, int H, std::initializer_list<const ppo2hip_seq *> seqs) {
-    int64_t reach = (64 * 2 - 1) / H + 1;
+    int64_t reach = (64 * k.V - 1) / H + 1;
     if (reach > E - 1) reach = E - 1;
     bool far = false;
     for (const ppo2hip_seq *s : seqs) far |= s && reach > 0 && s->e > ((1ll << 29) - 1 - H) / reach;
     if (!far) return;
     k.env_tiles = (int)ceil_div(H, 64 * k.V);
-    k.run_env_tiles = (int)ceil_div(H, 64 * k.run_V);
     k.tiles = (int64_t)E * k.env_tiles;
-    k.run_tiles = (int64_t)E * k.run_env_tiles;
 }
 
-static size_t runs_bytes(const Cut &k, int64_t C) { return k.sh.shares > 1 ? align_up((size_t)(k.sh.segs + k.sh.shares) * 3 * C * sizeof(float), 256) : 0; }
-static void place_runs(Cut &k, int64_t C, void *workspace) {
-    k.sh.seg_runs = (float *)workspace;
-    k.sh.share_runs = (float *)workspace + (int64_t)k.sh.segs * 3 * C;
+// words of a chain behind its counter
+static int64_t chain_words(const Cut &k, int64_t C) { return (3 * k.batches + ceil_div(k.batches, kGroup)) * C; }
+static size_t chain_bytes(const Cut &k, int64_t C) { return k.how == Cut::kChain ? 256 + align_up((size_t)chain_words(k, C) * sizeof(float), 256) : 0; }
+static int chain_begin(const Cut &k, int64_t C, void *workspace, Chain &ch, hipStream_t s) {
+    ch.turn = (unsigned *)workspace;
+    ch.runs = (float *)((char *)workspace + 256);
+    ch.states = ch.runs + 3 * k.batches * C;
+    ch.tiles = (unsigned)k.tiles;
+    ch.batches = k.batches;
+    // polls before a waiting wave gives up, about a second; PPO2HIP_GRID_SYNC_SPINS overrides it (negative: at once)
+    static const int spins = getenv("PPO2HIP_GRID_SYNC_SPINS") ? atoi(getenv("PPO2HIP_GRID_SYNC_SPINS")) : (1 << 20);
+    ch.max_spins = spins;
+    ch.fault = fault_word();
+    if (!ch.fault) return PPO2HIP_EINVAL;
+    const int64_t words = chain_words(k, C);
+    hipLaunchKernelGGL(glr_chain_clear_kernel, dim3((unsigned)ceil_div(words, 1024)), dim3(256), 0, s, ch, words);
+    return check_launch("glr_chain_clear_kernel");
 }
 
 extern "C" size_t ppo2hip_glr_forward_workspace_bytes(int dtype, int T, int E, int H) {
     if (T <= 1 || E <= 0 || H <= 0) return 0;
-    return runs_bytes(cut_of(dtype, T, E, H, false), (int64_t)E * H);
+    return chain_bytes(cut_of(dtype, T, E, H, false), (int64_t)E * H);
 }
 
 extern "C" size_t ppo2hip_glr_backward_workspace_bytes(int dtype, int T, int E, int H, int want_dbias) {
     if (T <= 0 || E <= 0 || H <= 0) return 0;
     const Cut k = cut_of(dtype, T, E, H, true);
-    const int64_t C = (int64_t)E * H, rows = (int64_t)k.sh.segs * E;
-    size_t n = runs_bytes(k, C);
+    const int64_t C = (int64_t)E * H, rows = (int64_t)k.batches * E;
+    size_t n = chain_bytes(k, C);
     if (want_dbias) n += align_up((size_t)rows * H * sizeof(float), 256) + align_up((size_t)ceil_div(rows, kSumRows) * H * sizeof(float), 256);
     return n;
 }
 
-template <class T, bool BACK>
-static int launch_runs(const Cut &k, const Seq<const T> &f, const Seq<const T> &x, const float *bias, const Seq<const uint8_t> &resets, int T_,
-                       unsigned C, unsigned H, hipStream_t s) {
-    const dim3 grid((unsigned)k.run_tiles, k.sh.segs), block(64 * kWaves);
-    if (sizeof(T) == 2 && k.run_V == 2)
-        hipLaunchKernelGGL((glr_runs_kernel<T, sizeof(T) == 2 ? 2 : 1, BACK>), grid, block, 0, s, f, x, bias, resets, T_, C, H, k.run_env_tiles, k.sh);
-    else
-        hipLaunchKernelGGL((glr_runs_kernel<T, 1, BACK>), grid, block, 0, s, f, x, bias, resets, T_, C, H, k.run_env_tiles, k.sh);
-    return check_launch("glr_runs_kernel");
-}
-
 template <class T, int V>
 static int forward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias, const ppo2hip_seq *resets, const float *h0,
-                      const ppo2hip_seq *y, float *h_last, float *saved, int T_, int E, int H, hipStream_t s) {
+                      const ppo2hip_seq *y, float *h_last, float *saved, void *workspace, int T_, int E, int H, hipStream_t s) {
     const int64_t C = (int64_t)E * H;
     if (T_ == 1) {
         hipLaunchKernelGGL((glr_step_kernel<T, V>), dim3((unsigned)ceil_div(C, 256 * V)), dim3(256), 0, s, seq_of<const T>(f), seq_of<const T>(x),
@@ -898,15 +1009,18 @@ static int forward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, 
     }
     const ForwardArgs<T> a = {seq_of<const T>(f), seq_of<const T>(x), seq_of<const uint8_t>(resets), seq_of<T>(y), bias, h0, h_last, saved,
                               T_, (unsigned)C, (unsigned)H, (unsigned)k.env_tiles};
-    if (k.held) {
-        hipLaunchKernelGGL((glr_forward_held_kernel<T, 1>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
+    if (k.how == Cut::kHold) {
+        hipLaunchKernelGGL((glr_forward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
         return check_launch("glr_forward_held_kernel");
     }
-    if (k.sh.shares > 1) {
-        int rc = launch_runs<T, false>(k, a.f, a.x, bias, a.resets, T_, a.C, a.H, s);
+    if (k.how == Cut::kChain) {
+        Chain ch;
+        int rc = chain_begin(k, C, workspace, ch, s);
         if (rc) return rc;
+        hipLaunchKernelGGL((glr_forward_chain_kernel<T, V>), dim3((unsigned)(k.tiles * k.batches)), dim3(64 * kChainWaves), 0, s, a, ch);
+        return check_launch("glr_forward_chain_kernel");
     }
-    hipLaunchKernelGGL((glr_forward_kernel<T, V>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * (k.sh.shares > 1 ? kWaves : 1)), 0, s, a, k.sh);
+    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((glr_forward_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64), 0, s, a);
     return check_launch("glr_forward_kernel");
 }
 
@@ -929,34 +1043,38 @@ extern "C" int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip
     }
     Cut k = cut_of(dtype, T, E, H, false);
     place_envs(k, E, H, {f, x, resets, y});
-    PPO2HIP_REQUIRE(T == 1 || k.sh.shares == 1 || workspace, "glr_forward: workspace is null");
-    place_runs(k, C, workspace);
-#define PPO2HIP_GLR_FORWARD(type, V) forward_of<type, V>(k, f, x, bias, resets, h0, y, h_last, saved, T, E, H, s)
+    PPO2HIP_REQUIRE(T == 1 || chain_bytes(k, C) == 0 || workspace, "glr_forward: workspace is null");
+    PPO2HIP_REQUIRE((uintptr_t)workspace % 16 == 0, "glr_forward: workspace must be aligned to 16 bytes");
+#define PPO2HIP_GLR_FORWARD(type, V) forward_of<type, V>(k, f, x, bias, resets, h0, y, h_last, saved, workspace, T, E, H, s)
     if (dtype == PPO2HIP_F32) return PPO2HIP_GLR_FORWARD(float, 1);
     if (dtype == PPO2HIP_BF16) return k.V == 2 ? PPO2HIP_GLR_FORWARD(__bf16, 2) : PPO2HIP_GLR_FORWARD(__bf16, 1);
     return k.V == 2 ? PPO2HIP_GLR_FORWARD(_Float16, 2) : PPO2HIP_GLR_FORWARD(_Float16, 1);
 #undef PPO2HIP_GLR_FORWARD
 }
 
-template <class T, int V>
+template <class T>
 static int backward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias, const ppo2hip_seq *resets, const float *saved,
                        const ppo2hip_seq *dy, const float *dh_last, const ppo2hip_seq *df, const ppo2hip_seq *dx, float *dbias, float *dh0,
                        void *workspace, int T_, int E, int H, hipStream_t s) {
-    const int64_t C = (int64_t)E * H, rows = (int64_t)k.sh.segs * E;
-    float *sums = (float *)((char *)workspace + runs_bytes(k, C));
+    const int64_t C = (int64_t)E * H, rows = (int64_t)k.batches * E;
+    float *sums = (float *)((char *)workspace + chain_bytes(k, C));
     const BackwardArgs<T> a = {seq_of<const T>(f), seq_of<const T>(x), seq_of<const T>(dy), seq_of<const uint8_t>(resets), seq_of<T>(df), seq_of<T>(dx),
                                bias, saved, dh_last, dbias ? sums : nullptr, dh0, T_, (unsigned)C, (unsigned)H, (unsigned)k.env_tiles};
     int rc;
-    if (k.held) {
-        hipLaunchKernelGGL((glr_backward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
+    if (k.how == Cut::kHold) {
+        hipLaunchKernelGGL((glr_backward_held_kernel<T>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
         rc = check_launch("glr_backward_held_kernel");
+    } else if (k.how == Cut::kChain) {
+        Chain ch;
+        if ((rc = chain_begin(k, C, workspace, ch, s))) return rc;
+        hipLaunchKernelGGL((glr_backward_chain_kernel<T>), dim3((unsigned)(k.tiles * k.batches)), dim3(64 * kChainWaves), 0, s, a, ch);
+        rc = check_launch("glr_backward_chain_kernel");
     } else {
-        if (k.sh.shares > 1 && (rc = launch_runs<T, true>(k, a.f, a.dy, bias, a.resets, T_, a.C, a.H, s))) return rc;
-        hipLaunchKernelGGL((glr_backward_kernel<T, V>), dim3((unsigned)k.tiles, k.sh.segs), dim3(64 * (k.sh.shares > 1 ? kWaves : 1)), 0, s, a, k.sh);
+        if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((glr_backward_kernel<T>), dim3((unsigned)k.tiles), dim3(64), 0, s, a);
         rc = check_launch("glr_backward_kernel");
     }
     if (rc || !dbias) return rc;
-    // rows [segment][env] of H channels each, kSumRows of them to a workgroup, until one row is left
+    // rows [batch][env] of H channels each, kSumRows of them to a workgroup, until one row is left
     float *in = sums, *out = (float *)((char *)sums + align_up((size_t)rows * H * sizeof(float), 256));
     for (int64_t n = rows;;) {
         const int64_t left = ceil_div(n, kSumRows);
@@ -992,9 +1110,9 @@ extern "C" int ppo2hip_glr_backward(int dtype, int T, int E, int H, const ppo2hi
     }
     Cut k = cut_of(dtype, T, E, H, true);
     place_envs(k, E, H, {f, x, resets, dy, df, dx});
-    PPO2HIP_REQUIRE((!dbias && k.sh.shares == 1) || workspace, "glr_backward: workspace is null");
-    place_runs(k, C, workspace);
-#define PPO2HIP_GLR_BACKWARD(type) backward_of<type, 1>(k, f, x, bias, resets, saved, dy, dh_last, df, dx, dbias, dh0, workspace, T, E, H, s)
+    PPO2HIP_REQUIRE((!dbias && chain_bytes(k, C) == 0) || workspace, "glr_backward: workspace is null");
+    PPO2HIP_REQUIRE((uintptr_t)workspace % 16 == 0, "glr_backward: workspace must be aligned to 16 bytes");
+#define PPO2HIP_GLR_BACKWARD(type) backward_of<type>(k, f, x, bias, resets, saved, dy, dh_last, df, dx, dbias, dh0, workspace, T, E, H, s)
     if (dtype == PPO2HIP_F32) return PPO2HIP_GLR_BACKWARD(float);
     if (dtype == PPO2HIP_BF16) return PPO2HIP_GLR_BACKWARD(__bf16);
     return PPO2HIP_GLR_BACKWARD(_Float16);

@@ -87,7 +87,7 @@ def check(hip, a, normal, dtype, kind="apart", dh_last=True, backward=True):
 
 SIZES = [(1, 1, 1), (1, 37, 333), (2, 3, 5), (15, 2, 64), (16, 1, 128), (17, 4, 65), (31, 1, 200), (33, 5, 7), (64, 1, 1), (100, 3, 130),
          (255, 2, 96), (256, 1, 64), (257, 2, 64), (513, 2, 70), (1001, 7, 33), (2049, 1, 258), (5000, 1, 64), (3, 300, 256), (128, 64, 256),
-         (40, 1, 2048), (777, 1, 1000)]
+         (40, 1, 2048), (777, 1, 1000), (9001, 1, 70), (12293, 2, 33), (4096, 1, 64), (4097, 3, 50), (300, 200, 256)]
 
 
 @pytest.mark.parametrize("T,E,H", SIZES)
@@ -150,7 +150,7 @@ def test_masks_that_leave_nothing(hip, T, dtype):
     check(hip, a, normal, dtype)
 
 
-@pytest.mark.parametrize("T", [5, 40, 700])
+@pytest.mark.parametrize("T", [5, 40, 700, 9000])
 def test_what_a_reset_hides_has_no_influence(hip, T):
     """A first state and inputs that are not numbers, in front of a reset: nothing of them behind it, in either direction."""
     E, H, r = 2, 70, T // 2
@@ -207,7 +207,7 @@ def test_gates_at_their_ends(hip, T):
     close(dh0, w0, tol, "dh0")
 
 
-@pytest.mark.parametrize("T", [4, 40, 600])
+@pytest.mark.parametrize("T", [4, 40, 600, 9000])
 def test_infinities_and_nans_follow_the_formula(hip, T):
     f = torch.zeros(T, 1, 8, device="cuda")
     x = torch.ones(T, 1, 8, device="cuda")
@@ -290,7 +290,7 @@ def test_state_may_be_none_of_the_outputs(hip):
         hip.glr_forward(torch.zeros(2, 3, 8), torch.zeros(2, 3, 8, device="cuda"))
 
 
-@pytest.mark.parametrize("T,E,H", [(600, 2, 130), (5000, 1, 64), (20, 300, 64)])
+@pytest.mark.parametrize("T,E,H", [(600, 2, 130), (20000, 1, 64), (20, 300, 64), (40, 200, 256)])
 def test_same_bits_every_time(hip, T, E, H):
     a, normal = make(T, E, H, BF16, resets=True, bias=True)
     dy = normal(T, E, H).to(BF16)
@@ -325,8 +325,8 @@ def test_gradients_against_differences(hip):
         assert abs(diff - want) < 2e-2 * (1 + abs(want)), (k, diff, want)
 
 
-def test_another_stream(hip):
-    T, E, H = 400, 3, 200
+@pytest.mark.parametrize("T,E,H", [(6000, 3, 200), (30, 200, 256)])
+def test_another_stream(hip, T, E, H):
     a, normal = make(T, E, H, BF16, resets=True, bias=True)
     dy = normal(T, E, H).to(BF16)
     want = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
@@ -343,7 +343,7 @@ def test_another_stream(hip):
         assert all(torch.equal(p, q) for p, q in zip(o, want[:2] + gwant))
 
 
-@pytest.mark.parametrize("T,E,H", [(1000, 1, 128), (40, 4, 64)])
+@pytest.mark.parametrize("T,E,H", [(9000, 1, 128), (40, 4, 64), (30, 200, 256)])
 def test_captured_and_replayed(hip, T, E, H):
     """Two graphs with their own workspaces, replayed in turn with eager work between, against eager results on new inputs."""
     a, normal = make(T, E, H, F32, resets=True, bias=True)
@@ -374,6 +374,24 @@ def test_captured_and_replayed(hip, T, E, H):
         torch.cuda.synchronize()
         for g, outs in graphs:
             assert all(torch.equal(p, q) for p, q in zip(outs, want)), k
+
+
+def test_envs_far_apart(hip):
+    """Envs 2^28 elements apart: a tile's lanes no longer reach them with 32-bit offsets."""
+    T, E, H = 300, 3, 34
+    se = 1 << 28
+    buf = torch.empty((E - 1) * se + T * H * 2 + 8, dtype=BF16, device="cuda")
+    views = [buf.as_strided((T, E, H), (2 * H, se, 1), k * H) for k in range(2)]
+    a, normal = make(T, E, H, BF16, resets=True, bias=True)
+    for v, t in zip(views, (a["f"], a["x"])):
+        v.copy_(t)
+    a["f"], a["x"] = views
+    check(hip, a, normal, BF16)
+    t, _ = make(20, E, H, BF16)
+    for v, w in zip(views, (t["f"], t["x"])):
+        v[:20].copy_(w)
+    a["f"], a["x"], a["resets"] = views[0][:20], views[1][:20], None
+    check(hip, a, normal, BF16)
 
 
 def test_offsets_beyond_32_bits(hip):
