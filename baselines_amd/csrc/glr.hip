@@ -253,9 +253,14 @@ __device__ inline unsigned anew(unsigned v) {
     return v;
 }
 
-// A span's gates and what each step adds to the state, u = (1 - a) x.  Steps behind the last one keep the state as it is.
+// A gate with a reset at its step is shut for the state: a finite one is multiplied by zero, a NaN stays one.
+template <bool EXACT>
+__device__ inline float with_reset(float g, unsigned rm, int i) { return rm >> i & 1 ? Gate<EXACT>::shut() : g; }
+
+// A span's gates, shut at resets, and what each step adds to the state, u = (1 - a) x of the gate itself.  Steps behind the last
+// one keep the state as it is.
 template <class T, int V>
-__device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, Span<V> &g, Span<V> &u) {
+__device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, unsigned rm, Span<V> &g, Span<V> &u) {
     typedef Gate<sizeof(T) == 4> G;
 #pragma unroll
     for (int i = 0; i < kSpan; i++)
@@ -270,6 +275,11 @@ __device__ inline void span_open(const Raw<T, V> &f, const Raw<T, V> &x, const f
 #pragma unroll
             for (int k = 0; k < V; k++)
                 if (i >= n) g[i][k] = G::open(), u[i][k] = 0.f;
+    if (__any(rm != 0))
+#pragma unroll
+        for (int i = 0; i < kSpan; i++)
+#pragma unroll
+            for (int k = 0; k < V; k++) g[i][k] = with_reset<sizeof(T) == 4>(g[i][k], rm, i);
 }
 
 template <int V>
@@ -280,13 +290,13 @@ __device__ inline bool any_not_finite(const float (&h)[V]) {
     return __any(bad);
 }
 
-// Walks a span from state h, handing every step's state to `out(i, h)`: the quick way where no lane has a reset and `whole` says
-// that out may be called for all steps, the general way (out only for steps below n) elsewhere.  The quick form of a step turns an
-// infinite state to NaN, which then stays to the span's end: the span is walked again.
+// Walks a span from state h, handing every step's state to `out(i, h)`: the quick way where `whole` says that out may be called for
+// all steps, the general way (out only for steps below n) elsewhere.  The quick form of a step turns an infinite state to NaN, and
+// NaN goes through shut gates: a span that met either ends in NaN and is walked again.
 template <bool EXACT, int V, class Out>
 __device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm, bool whole, int n, float (&h)[V], Out out) {
     typedef Gate<EXACT> G;
-    if (whole && !__any(rm != 0)) {
+    if (whole) {
         float h0[V];
 #pragma unroll
         for (int k = 0; k < V; k++) h0[k] = h[k];
@@ -347,10 +357,13 @@ __device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsi
     if (!__any(rm != 0)) {
 #pragma unroll
         for (int i = kSpan - 1; i >= 0; i--) c[0] = G::pass(g[i][0], c[0] + dy.get(i, 0));
-        r[0].B = c[0];
-        if (!any_not_finite(c)) return;
-        c[0] = 0.f;
+    } else {
+#pragma unroll
+        for (int i = kSpan - 1; i >= 0; i--) c[0] = G::pass(with_reset<sizeof(T) == 4>(g[i][0], rm, i), c[0] + dy.get(i, 0));
     }
+    r[0].B = c[0];
+    if (!any_not_finite(c)) return;
+    c[0] = 0.f;
 #pragma unroll
     for (int i = kSpan - 1; i >= 0; i--) c[0] = anew(rm) >> i & 1 ? 0.f : G::pass_any(anew(g[i][0]), c[0] + dy.get(i, 0));
     r[0].B = c[0];
@@ -368,7 +381,7 @@ __device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsi
 // for the runs of its group's earlier batches and for the state in front of the group: what is joined with what does not depend
 // on who came first, so that results are the same bits every time.
 // A word is published by one agent-scope store and is its own flag: a launch before fills all words with kEmpty, a NaN that no
-// arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with zeros.
+// arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with NaN.
 constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan, kGroup = 32;
 constexpr unsigned kEmpty = 0xffffffffu;
 
@@ -427,7 +440,7 @@ __device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned
             publish(o, all.A), publish(o + C, all.D), publish(o + 2 * (int64_t)C, all.B);
         }
     }
-    const unsigned byte = at.c * 4u;                      // a chain has few columns
+    const unsigned byte = at.c * 4u;                      // C < 2^30
     // the group's earlier batches, up to kEach to a wave
     constexpr int kEach = kGroup / kChainWaves;
     const int lo = w * kEach;
@@ -451,7 +464,7 @@ __device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned
                 for (int q = 0; q < 3; q++)
 #pragma unroll
                     for (int k = 0; k < V; k++) ok &= bits[i][q][k] != kEmpty;
-            if (__all(ok)) break;
+            if (__all(ok) && ch.max_spins >= 0) break;
             if (tries >= ch.max_spins) {
                 if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
                 break;
@@ -476,7 +489,7 @@ __device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned
                 for (int k = 0; k < V; k++) bits[k] = peek(ch.states + (int64_t)group * C + k, byte);
 #pragma unroll
                 for (int k = 0; k < V; k++) ok &= bits[k] != kEmpty;
-                if (__all(ok)) break;
+                if (__all(ok) && ch.max_spins >= 0) break;
                 if (tries >= ch.max_spins) {
                     if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
                     break;
@@ -581,7 +594,7 @@ __device__ inline void forward_walk(const ForwardArgs<T> &a, const Place &at, in
         const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
         const unsigned rm = span_resets(a.resets, t0, n, at);
         Span<V> g, u;
-        span_open<T, V>(fr, xr, b, n, g, u);
+        span_open<T, V>(fr, xr, b, n, rm, g, u);
         if (span + 1 < end) fetch(span + 1);
         forward_span<T, V>(a, at, yo, t0, n, rm, g, u, h);
     }
@@ -615,7 +628,7 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
     for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f;
     Span<V> g, u;
     Run r[V];
-    span_open<T, V>(fr, xr, b, n, g, u);
+    span_open<T, V>(fr, xr, b, n, rm, g, u);
     span_run<sizeof(T) == 4, V>(g, u, rm, r);
 #pragma unroll
     for (int k = 0; k < V; k++) {
@@ -643,7 +656,7 @@ __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_
     for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[d.at.j + k] : 0.f;
     Span<V> g, u;
     Run r[V];
-    span_open<T, V>(fr, xr, b, d.n, g, u);
+    span_open<T, V>(fr, xr, b, d.n, rm, g, u);
     span_run<sizeof(T) == 4, V>(g, u, rm, r);
 #pragma unroll
     for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[d.at.c + k] : 0.f;
@@ -670,8 +683,8 @@ struct BackwardArgs {
 template <class T>
 __device__ inline void back_open(const Raw<T, 1> &f, const Raw<T, 1> &x, float b, float kept, int n, unsigned rm, Span<1> &g, Span<1> &q) {
     typedef Gate<sizeof(T) == 4> G;
+    constexpr bool kExact = sizeof(T) == 4;
     float h[1] = {kept}, slope;
-    bool done = false;
     if (!__any(rm != 0)) {
 #pragma unroll
         for (int i = 0; i < kSpan; i++) {
@@ -680,9 +693,16 @@ __device__ inline void back_open(const Raw<T, 1> &f, const Raw<T, 1> &x, float b
             q[i][0] = (h[0] - xv) * slope;
             h[0] = G::pass(v, h[0]) + G::take(v) * xv;
         }
-        done = !any_not_finite(h);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSpan; i++) {
+            const float xv = x.get(i, 0), v = G::of(f.get(i, 0) + b, slope);
+            g[i][0] = v;
+            q[i][0] = ((rm >> i & 1 ? 0.f : h[0]) - xv) * slope;
+            h[0] = G::pass(with_reset<kExact>(v, rm, i), h[0]) + G::take(v) * xv;
+        }
     }
-    if (!done) {
+    if (any_not_finite(h)) {
         h[0] = kept;
 #pragma unroll
         for (int i = 0; i < kSpan; i++) {
@@ -716,16 +736,27 @@ __device__ inline void back_span(const BackwardArgs<T> &a, const Place &at, unsi
             Lane<T, 1>::store(xp + here(dxo), x1);
         }
     };
+    constexpr bool kExact = sizeof(T) == 4;
     float sum = 0.f, c[1] = {in};
     bool done = false;
-    if (n >= kSpan && !__any(rm != 0)) {
+    if (n >= kSpan) {
         n = kSpan;
+        if (!__any(rm != 0)) {
 #pragma unroll
-        for (int i = kSpan - 1; i >= 0; i--) {
-            const float gs = dy.get(i, 0) + c[0], of = gs * q[i][0];
-            sum += of;
-            put(i, of, G::take(g[i][0]) * gs);
-            c[0] = G::pass(g[i][0], gs);
+            for (int i = kSpan - 1; i >= 0; i--) {
+                const float gs = dy.get(i, 0) + c[0], of = gs * q[i][0];
+                sum += of;
+                put(i, of, G::take(g[i][0]) * gs);
+                c[0] = G::pass(g[i][0], gs);
+            }
+        } else {
+#pragma unroll
+            for (int i = kSpan - 1; i >= 0; i--) {
+                const float gs = dy.get(i, 0) + c[0], of = gs * q[i][0];
+                sum += of;
+                put(i, of, G::take(g[i][0]) * gs);
+                c[0] = G::pass(with_reset<kExact>(g[i][0], rm, i), gs);
+            }
         }
         done = !any_not_finite(c);
     }
@@ -871,12 +902,13 @@ __global__ __launch_bounds__(256) void glr_step_kernel(Seq<const T> f, Seq<const
         for (int k = 0; k < V; k++) h_last[c + k] = h[k];
 }
 
-// Column sums of in [rows, H]: workgroup (i, r) sums rows r * kSumRows .. of 32 columns, 32 rows side by side, into out[r, H]
+// Column sums of in [rows, H]: a workgroup sums kSumRows rows of 32 columns, 32 rows side by side, into a row of out
 constexpr int kSumRows = 2048;
 __global__ __launch_bounds__(1024) void glr_column_sum_kernel(const float *__restrict__ in, int64_t rows, int H, float *__restrict__ out) {
     __shared__ double red[32][33];
-    const int col = threadIdx.x & 31, grp = threadIdx.x >> 5, j = blockIdx.x * 32 + col;
-    const int64_t r0 = (int64_t)blockIdx.y * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
+    const unsigned across = (unsigned)(H + 31) / 32, part = blockIdx.x / across;
+    const int col = threadIdx.x & 31, grp = threadIdx.x >> 5, j = (int)(blockIdx.x - part * across) * 32 + col;
+    const int64_t r0 = (int64_t)part * kSumRows, r1 = r0 + kSumRows < rows ? r0 + kSumRows : rows;
     double s = 0.0;
     if (j < H)
 #pragma unroll 8
@@ -887,7 +919,7 @@ __global__ __launch_bounds__(1024) void glr_column_sum_kernel(const float *__res
         s = 0.0;
 #pragma unroll
         for (int g = 0; g < 32; g++) s += red[g][col];
-        out[(int64_t)blockIdx.y * H + j] = (float)s;
+        out[(int64_t)part * H + j] = (float)s;
     }
 }
 
@@ -911,6 +943,7 @@ static int glr_check(const char *what, int dtype, int T, int E, int H) {
     PPO2HIP_REQUIRE(dtype == PPO2HIP_F32 || dtype == PPO2HIP_BF16 || dtype == PPO2HIP_F16, "%s: unknown dtype %d", what, dtype);
     PPO2HIP_REQUIRE(T >= 0 && E >= 0 && H >= 0, "%s: negative size T=%d E=%d H=%d", what, T, E, H);
     PPO2HIP_REQUIRE((int64_t)E * H <= 0x7fffffffll, "%s: E*H=%lld beyond 2^31 - 1 columns", what, (long long)E * H);
+    PPO2HIP_REQUIRE(H < 1 << 26, "%s: H=%d beyond 2^26 - 1 channels", what, H);           // lanes' offsets and launches stay within 32 bits
     return PPO2HIP_OK;
 }
 
@@ -933,7 +966,8 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
 
 // How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile, walked by
 // one wave per tile, or passed along a chain of workgroups.  Measured, us forward / backward:
-//   [128, E, H] float32, 1024 tiles: held 18.5 / 29.2, walked 21.6 / 35.4; 4096 tiles: 83 / 138, 86 / 138
+//   [128, E, H] float32, 1024 tiles: held 20.9 / 38, walked 25.9 / 37.5; 4096 tiles: 84 / 141, 90 / 149
+//   [256, E, H] bfloat16, 512 tiles: held 26 / 47, walked 34 / 50; 1024: 49 / 95, 49 / 79; 4096: 180 / 385, 179 / 307
 //   [2048, E, H] float32, 384 tiles: chain 125 / 197, walked 226 / 491; 2048 tiles: 624 / 1056, 688 / 1127
 //   [512, E, H] bfloat16, 768 tiles: chain 75 / 140, walked 72 / 139; 1024: 97 / 185, 87 / 152; 4096: 365 / 718, 347 / 583
 struct Cut {
@@ -945,7 +979,8 @@ static Cut cut_of(int dtype, int T, int E, int H, bool back) {
     Cut k;
     const int64_t C = (int64_t)E * H;
     const int wide = dtype != PPO2HIP_F32 && H % 2 == 0 ? 2 : 1;
-    k.how = T <= kHeld * kSpan ? Cut::kHold : dtype != PPO2HIP_F32 && ceil_div(C, 64 * wide) >= kWalkTiles ? Cut::kWalk : Cut::kChain;
+    const bool many = dtype != PPO2HIP_F32 && ceil_div(C, 64 * wide) >= kWalkTiles, few = T <= kHeld * kSpan;
+    k.how = many && (back || !few) ? Cut::kWalk : few ? Cut::kHold : Cut::kChain;
     // two channels per lane halve a 16-bit sequence's loads and double what is in flight; going back there are no registers for them
     k.V = back ? 1 : wide;
     k.tiles = ceil_div(C, 64 * k.V);
@@ -965,6 +1000,15 @@ static void place_envs(Cut &k, int E, int H, std::initializer_list<const ppo2hip
     k.tiles = (int64_t)E * k.env_tiles;
 }
 
+static unsigned threads_of(const Cut &k, int T) {
+    return 64 * (unsigned)(k.how == Cut::kHold ? ceil_div(T, kSpan) : k.how == Cut::kChain ? kChainWaves : 1);
+}
+static int cut_check(const char *what, const Cut &k, int T, int64_t C) {
+    PPO2HIP_REQUIRE(k.tiles * k.batches <= (int64_t)(0xffffffffu / threads_of(k, T)), "%s: T=%d, %lld columns: beyond one launch", what, T, (long long)C);
+    PPO2HIP_REQUIRE(k.how != Cut::kChain || C < 1ll << 30, "%s: T=%d, %lld columns: beyond 2^30 - 1 for so many steps", what, T, (long long)C);
+    return PPO2HIP_OK;
+}
+
 // words of a chain behind its counter
 static int64_t chain_words(const Cut &k, int64_t C) { return (3 * k.batches + ceil_div(k.batches, kGroup)) * C; }
 static size_t chain_bytes(const Cut &k, int64_t C) { return k.how == Cut::kChain ? 256 + align_up((size_t)chain_words(k, C) * sizeof(float), 256) : 0; }
@@ -974,7 +1018,7 @@ static int chain_begin(const Cut &k, int64_t C, void *workspace, Chain &ch, hipS
     ch.states = ch.runs + 3 * k.batches * C;
     ch.tiles = (unsigned)k.tiles;
     ch.batches = k.batches;
-    // polls before a waiting wave gives up, about a second; PPO2HIP_GRID_SYNC_SPINS overrides it (negative: at once)
+    // polls before a waiting wave gives up, about a second; PPO2HIP_GRID_SYNC_SPINS overrides it (negative: the first poll already counts as given up)
     static const int spins = getenv("PPO2HIP_GRID_SYNC_SPINS") ? atoi(getenv("PPO2HIP_GRID_SYNC_SPINS")) : (1 << 20);
     ch.max_spins = spins;
     ch.fault = fault_word();
@@ -1010,7 +1054,7 @@ static int forward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, 
     const ForwardArgs<T> a = {seq_of<const T>(f), seq_of<const T>(x), seq_of<const uint8_t>(resets), seq_of<T>(y), bias, h0, h_last, saved,
                               T_, (unsigned)C, (unsigned)H, (unsigned)k.env_tiles};
     if (k.how == Cut::kHold) {
-        hipLaunchKernelGGL((glr_forward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
+        hipLaunchKernelGGL((glr_forward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(threads_of(k, T_)), 0, s, a);
         return check_launch("glr_forward_held_kernel");
     }
     if (k.how == Cut::kChain) {
@@ -1043,6 +1087,7 @@ extern "C" int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip
     }
     Cut k = cut_of(dtype, T, E, H, false);
     place_envs(k, E, H, {f, x, resets, y});
+    if ((rc = cut_check("glr_forward", k, T, C))) return rc;
     PPO2HIP_REQUIRE(T == 1 || chain_bytes(k, C) == 0 || workspace, "glr_forward: workspace is null");
     PPO2HIP_REQUIRE((uintptr_t)workspace % 16 == 0, "glr_forward: workspace must be aligned to 16 bytes");
 #define PPO2HIP_GLR_FORWARD(type, V) forward_of<type, V>(k, f, x, bias, resets, h0, y, h_last, saved, workspace, T, E, H, s)
@@ -1062,7 +1107,7 @@ static int backward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x,
                                bias, saved, dh_last, dbias ? sums : nullptr, dh0, T_, (unsigned)C, (unsigned)H, (unsigned)k.env_tiles};
     int rc;
     if (k.how == Cut::kHold) {
-        hipLaunchKernelGGL((glr_backward_held_kernel<T>), dim3((unsigned)k.tiles), dim3(64 * (unsigned)ceil_div(T_, kSpan)), 0, s, a);
+        hipLaunchKernelGGL((glr_backward_held_kernel<T>), dim3((unsigned)k.tiles), dim3(threads_of(k, T_)), 0, s, a);
         rc = check_launch("glr_backward_held_kernel");
     } else if (k.how == Cut::kChain) {
         Chain ch;
@@ -1078,7 +1123,7 @@ static int backward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x,
     float *in = sums, *out = (float *)((char *)sums + align_up((size_t)rows * H * sizeof(float), 256));
     for (int64_t n = rows;;) {
         const int64_t left = ceil_div(n, kSumRows);
-        hipLaunchKernelGGL(glr_column_sum_kernel, dim3((unsigned)ceil_div(H, 32), (unsigned)left), dim3(1024), 0, s, in, n, H, left == 1 ? dbias : out);
+        hipLaunchKernelGGL(glr_column_sum_kernel, dim3((unsigned)(ceil_div(H, 32) * left)), dim3(1024), 0, s, in, n, H, left == 1 ? dbias : out);
         if ((rc = check_launch("glr_column_sum_kernel")) || left == 1) return rc;
         float *t = in;
         in = out, out = t, n = left;
@@ -1110,6 +1155,7 @@ extern "C" int ppo2hip_glr_backward(int dtype, int T, int E, int H, const ppo2hi
     }
     Cut k = cut_of(dtype, T, E, H, true);
     place_envs(k, E, H, {f, x, resets, dy, df, dx});
+    if ((rc = cut_check("glr_backward", k, T, C))) return rc;
     PPO2HIP_REQUIRE((!dbias && chain_bytes(k, C) == 0) || workspace, "glr_backward: workspace is null");
     PPO2HIP_REQUIRE((uintptr_t)workspace % 16 == 0, "glr_backward: workspace must be aligned to 16 bytes");
 #define PPO2HIP_GLR_BACKWARD(type) backward_of<type>(k, f, x, bias, resets, saved, dy, dh_last, df, dx, dbias, dh0, workspace, T, E, H, s)

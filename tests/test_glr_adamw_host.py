@@ -168,3 +168,31 @@ def test_c_entry_refuses_bad_lists(_lib):
     assert step(clip=1.0) == _lib.ENOSPACE
     assert L.ppo2hip_adamw_state(good, 2, one, one, one, one, one, 2, one, one, None) == _lib.EINVAL
     assert L.ppo2hip_adamw_state(good, 2, one, one, None, one, one, 0, one, one, None) == _lib.EINVAL
+
+
+def test_c_entry_refuses_what_a_launch_or_a_lane_cannot_address(_lib):
+    """Lanes carry 32-bit byte offsets and a launch 2^32 threads: sizes beyond either are refused before anything runs."""
+    L, one = _lib.lib, ctypes.c_void_p(256)
+    seq = _lib.Seq(256, 0, 0)
+    fwd = lambda T, E, H, dt=0: L.ppo2hip_glr_forward(dt, T, E, H, seq, seq, None, None, None, seq, None, None, one, 1 << 62, None)      # noqa: E731
+    bwd = lambda T, E, H, dt=0: L.ppo2hip_glr_backward(      # noqa: E731
+        dt, T, E, H, seq, seq, None, None, one, seq, None, seq, seq, None, None, one, 1 << 62, None)
+    for call in (fwd, bwd):
+        for T, E, H in ((2, 1, 1 << 26), (1000, 31, (1 << 26) - 1), (1000, 1 << 30, 1), (1 << 30, 1 << 20, 1)):
+            assert call(T, E, H) == _lib.EINVAL and L.ppo2hip_last_error(), (T, E, H)
+    # tiles of 64 columns, a workgroup of 1024 threads each: 2^22 of them
+    assert fwd(256, 1 << 5, 1 << 23) == _lib.EINVAL and b"one launch" in L.ppo2hip_last_error()
+
+
+def test_c_entry_refuses_lists_and_norms_that_do_not_fit(_lib):
+    L, one = _lib.lib, ctypes.c_void_p(256)
+    T = _lib.AdamwTensor
+    long = (T * 2)(T(256, 1 << 34, 0, 0, 1.0, 0), T(4096, 1 << 34, 0, 0, 1.0, 0))
+    assert L.ppo2hip_adamw_state_elements(long, 1, 32) == 1 << 34
+    assert L.ppo2hip_adamw_state_elements(long, 2, 32) == _lib.EINVAL and b"elements in one list" in L.ppo2hip_last_error()
+    good, grads = (T * 1)(T(256, 300, 0, 0, 1.0, 0)), (ctypes.c_void_p * 1)(256)
+    step = lambda clip, plan=one, ws=one: L.ppo2hip_adamw_step(      # noqa: E731
+        good, 1, 32, plan, grads, one, None, one, None, 1e-3, 1, .9, .999, 1e-8, 0.0, 1.0, clip, None, ws, 1 << 20, None)
+    for clip in (1e-60, float("nan")):
+        assert step(clip) == _lib.EINVAL and b"max_grad_norm" in L.ppo2hip_last_error()
+    assert step(1.0, ws=ctypes.c_void_p(264)) == _lib.EINVAL and step(1.0, plan=ctypes.c_void_p(264)) == _lib.EINVAL

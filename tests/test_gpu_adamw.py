@@ -411,3 +411,22 @@ def test_training_a_recurrent_layer(hip):
     # Adam divides by the root of v: an element whose gradient is far below its tensor's norm may step any way within lr
     for got, want in zip((w, bias, head), wide):
         assert float((got.double() - want.detach()).norm() / want.detach().norm()) < 1e-3
+
+
+@pytest.mark.parametrize("sizes", [[700, 3], [40000]])
+@pytest.mark.parametrize("eps", [0.0, 1e-38, 1e-30, 1e-12, 1e-8, 1.0])
+@pytest.mark.parametrize("scale", [1e-15, 1.0])
+def test_small_and_large_epsilons(hip, sizes, eps, scale):
+    """Gradients whose squares are near the smallest normal numbers, with an epsilon on either side of their roots."""
+    g = torch.Generator(device="cuda").manual_seed(7)
+    ps = tensors(sizes, F32, g, 0.1)
+    plan = hip.AdamWPlan(ps)
+    lr = 1e-2
+    for t in (1, 2):
+        grads = [scale * torch.sign(x) * (0.5 + torch.rand(x.shape, generator=g, device="cuda")) for x in tensors(sizes, F32, g)]
+        old = [p.double() for p in ps]
+        m, v = ([s.double() for s in x.split(sizes)] for x in (plan.m, plan.v))
+        hip.adamw_step(plan, grads, lr, t, epsilon=eps, weight_decay=0.0, max_grad_norm=1e30)
+        (new, nm, nv, gs), _, _ = reference(old, grads, m, v, lr, t, [0] * len(sizes), wd=0.0, eps=eps)
+        for k in range(len(sizes)):
+            close(ps[k], new[k], tol_p(old[k], new[k], lr, m[k], nm[k], nv[k], t, gs[k]), ("p", k, t))

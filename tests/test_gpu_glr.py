@@ -405,3 +405,54 @@ def test_offsets_beyond_32_bits(hip):
         v.copy_(t)
     a["f"], a["x"] = views
     check(hip, a, normal, BF16)
+
+
+_GAVE_UP_SCRIPT = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from baselines_amd import _lib, hip
+T, E, H = 700, 2, 70
+f, x, dy = (torch.randn(T, E, H, device="cuda") for _ in range(3))
+seen = []
+def look(what):
+    torch.cuda.synchronize()
+    try:
+        hip.take_faults()
+    except _lib.Ppo2HipError as e:
+        seen.append(what + ": " + str(e))
+y, _, saved = hip.glr_forward(f, x, want_saved=True)
+look("forward")
+hip.glr_backward(f, x, dy, saved)
+look("backward")
+hip.glr_forward(f[:256], x[:256])
+look("held")
+print("SEEN", len(seen), seen)
+"""
+
+
+@pytest.mark.parametrize("forced", [False, True])
+def test_a_chain_that_gave_up_is_reported(tmp_path, forced):
+    """PPO2HIP_GRID_SYNC_SPINS=-1 makes every wait of the chain count as given up: both long passes raise the library's fault word
+    and end as usual, and a sequence that one workgroup holds, which waits for nobody, raises nothing."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "gave_up.py"
+    script.write_text(_GAVE_UP_SCRIPT)
+    env = dict(os.environ)
+    if forced:
+        env["PPO2HIP_GRID_SYNC_SPINS"] = "-1"
+    res = subprocess.run([sys.executable, str(script), root], env=env, capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0, res.stderr[-2000:]
+    line = [l for l in res.stdout.splitlines() if l.startswith("SEEN")][0]
+    assert line.startswith("SEEN 2" if forced else "SEEN 0"), line
+    assert not forced or ("forward" in line and "backward" in line and "gave up" in line)
+
+
+@pytest.mark.parametrize("T,E,H", [(1, 4100, 33), (2, 2049, 1), (300, 70, 65)])
+def test_bias_gradient_over_many_rows(hip, T, E, H):
+    """More rows of partial sums than one workgroup adds up, and columns that end inside a workgroup's 32."""
+    a, normal = make(T, E, H, F32, bias=True, seed=E)
+    check(hip, a, normal, F32)
