@@ -80,20 +80,44 @@ struct Gate<false> {
 // runs of steps
 // ---------------------------------------------------------------------------------------------------------------------
 
-// What a run of steps does to the state that enters it: h -> A h + B, with D = 1 - A kept beside A because a product of gates
-// next to one has lost D's figures; A < 0 marks a run with a reset in it, which lets nothing through, infinities and NaN included.
-// Going back in time the same three numbers carry the gradient that leaves a run at its front.
-struct Run {
-    float A, D, B;
+// What a run of steps does to the state that enters it: h -> A h + B, words of which are handed from wave to wave.  Going back in
+// time the same numbers carry the gradient that leaves a run at its front.
+template <bool EXACT>
+struct Run;
+
+// float32: A, D and B with D = 1 - A kept beside A because a product of gates next to one has lost D's figures; A < 0 marks a
+// run with a reset in it, which lets nothing through, infinities and NaN included.
+template <>
+struct Run<true> {
+    static constexpr int kWords = 3;
+    float w[3];
+    static __device__ inline Run none() { return {{1.f, 0.f, 0.f}}; }
+    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? -1.f : A, D, 0.f}}; }
+    __device__ inline void add(float B) { w[2] = B; }
+    __device__ inline float through(float h) const {
+        if (w[0] < 0.f) return w[2];
+        const float kept = w[1] <= 0.5f ? fmaf(-w[1], h, h) : w[0] * h;
+        return (fabsf(h) < INFINITY ? kept : h) + w[2];    // an infinite state stays one however small A became
+    }
+    // this run and then that one
+    __device__ inline Run join(const Run &r) const {
+        return {{r.w[0] < 0.f || w[0] < 0.f ? -1.f : w[0] * r.w[0], fmaf(1.f - w[1], r.w[1], w[1]), r.through(w[2])}};
+    }
 };
-__device__ inline float run_through(const Run &r, float h) {
-    if (r.A < 0.f) return r.B;
-    const float kept = r.D <= 0.5f ? fmaf(-r.D, h, h) : r.A * h;
-    return (fabsf(h) < INFINITY ? kept : h) + r.B;         // an infinite state stays one however small A became
-}
-__device__ inline Run run_join(const Run &first, const Run &then) {
-    return {then.A < 0.f || first.A < 0.f ? -1.f : first.A * then.A, fmaf(1.f - first.D, then.D, first.D), run_through(then, first.B)};
-}
+
+// 16 bits: A, rounded once from whichever of A and D has more figures, and B.  A is zero where a reset is, and else never: its
+// least value moves no finite state by as much as 5e-7 and keeps an infinite one.
+template <>
+struct Run<false> {
+    static constexpr int kWords = 2;
+    float w[2];
+    static __device__ inline float live(float A) { return fmaxf(A, 0x1p-149f); }
+    static __device__ inline Run none() { return {{1.f, 0.f}}; }
+    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? 0.f : live(D <= 0.5f ? 1.f - D : A), 0.f}}; }
+    __device__ inline void add(float B) { w[1] = B; }
+    __device__ inline float through(float h) const { return w[0] == 0.f ? w[1] : fmaf(w[0], h, w[1]); }
+    __device__ inline Run join(const Run &r) const { return {{r.w[0] == 0.f || w[0] == 0.f ? 0.f : live(w[0] * r.w[0]), r.through(w[1])}}; }
+};
 
 // ---------------------------------------------------------------------------------------------------------------------
 // addresses
@@ -318,39 +342,39 @@ __device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm
     }
 }
 
-// A and D of a span.  D grows by 1 - a of what is left of it, so that it keeps its figures while it is small.
+// What a span lets through.  D = 1 - A grows by 1 - a of what is left of it, so that it keeps its figures while it is small.
 template <bool EXACT, int V>
-__device__ inline void span_passes(const Span<V> &g, unsigned rm, Run (&r)[V]) {
+__device__ inline void span_passes(const Span<V> &g, unsigned rm, Run<EXACT> (&r)[V]) {
     typedef Gate<EXACT> G;
+    float A[V], D[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) r[k].A = 1.f, r[k].D = 0.f;
+    for (int k = 0; k < V; k++) A[k] = 1.f, D[k] = 0.f;
 #pragma unroll
     for (int i = 0; i < kSpan; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) {
             const float om = G::take(g[i][k]);
-            r[k].A = G::pass(g[i][k], r[k].A);
-            r[k].D = r[k].D + fmaf(-r[k].D, om, om);
+            A[k] = G::pass(g[i][k], A[k]);
+            D[k] = D[k] + fmaf(-D[k], om, om);
         }
 #pragma unroll
-    for (int k = 0; k < V; k++)
-        if (rm) r[k].A = -1.f;
+    for (int k = 0; k < V; k++) r[k] = Run<EXACT>::of(A[k], D[k], rm != 0);
 }
 
 // A span's run in the direction of time,
 template <bool EXACT, int V>
-__device__ inline void span_run(const Span<V> &g, const Span<V> &u, unsigned rm, Run (&r)[V]) {
+__device__ inline void span_run(const Span<V> &g, const Span<V> &u, unsigned rm, Run<EXACT> (&r)[V]) {
     float h[V];
 #pragma unroll
     for (int k = 0; k < V; k++) h[k] = 0.f;
     span_passes<EXACT, V>(g, rm, r);
     span_walk<EXACT, V>(g, u, rm, true, kSpan, h, [](int, const float (&)[V]) {});
 #pragma unroll
-    for (int k = 0; k < V; k++) r[k].B = h[k];
+    for (int k = 0; k < V; k++) r[k].add(h[k]);
 }
 // and against it, for the gradient: dy enters a step before the gate does, a reset stands behind it.
 template <class T>
-__device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsigned rm, Run (&r)[1]) {
+__device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsigned rm, Run<sizeof(T) == 4> (&r)[1]) {
     typedef Gate<sizeof(T) == 4> G;
     span_passes<sizeof(T) == 4, 1>(g, rm, r);
     float c[1] = {0.f};
@@ -361,13 +385,31 @@ __device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsi
 #pragma unroll
         for (int i = kSpan - 1; i >= 0; i--) c[0] = G::pass(with_reset<sizeof(T) == 4>(g[i][0], rm, i), c[0] + dy.get(i, 0));
     }
-    r[0].B = c[0];
+    r[0].add(c[0]);
     if (!any_not_finite(c)) return;
     c[0] = 0.f;
 #pragma unroll
     for (int i = kSpan - 1; i >= 0; i--) c[0] = anew(rm) >> i & 1 ? 0.f : G::pass_any(anew(g[i][0]), c[0] + dy.get(i, 0));
-    r[0].B = c[0];
+    r[0].add(c[0]);
 }
+
+// A tile's runs, as waves of a workgroup hand them on.
+template <bool EXACT, int V>
+struct RunSpace {
+    float w[Run<EXACT>::kWords][64 * V];
+    __device__ inline void put(const Run<EXACT> (&r)[V]) {
+#pragma unroll
+        for (int q = 0; q < Run<EXACT>::kWords; q++)
+#pragma unroll
+            for (int k = 0; k < V; k++) w[q][(threadIdx.x & 63) * V + k] = r[k].w[q];
+    }
+    __device__ inline Run<EXACT> get(int k) const {
+        Run<EXACT> r;
+#pragma unroll
+        for (int q = 0; q < Run<EXACT>::kWords; q++) r.w[q] = w[q][(threadIdx.x & 63) * V + k];
+        return r;
+    }
+};
 
 // ---------------------------------------------------------------------------------------------------------------------
 // a chain of workgroups
@@ -387,7 +429,7 @@ constexpr unsigned kEmpty = 0xffffffffu;
 
 struct Chain {
     unsigned *turn;         // the counter, in 256 bytes of its own; then
-    float *runs;            // [batches][A, D, B][C]
+    float *runs;            // [batches][words of a run][C]
     float *states;          // [groups][C]: in front of groups 1, 2, ...
     unsigned tiles;
     int batches, max_spins;
@@ -412,56 +454,58 @@ __global__ __launch_bounds__(256) void glr_chain_clear_kernel(Chain ch, int64_t 
         for (int k = 0; i + k < words; k++) p[k] = kEmpty;
 }
 
-template <int V>
+template <bool EXACT, int V>
 struct ChainSpace {
-    float runs[kChainWaves][3][64 * V], before[kChainWaves][3][64 * V], state[64 * V];
+    RunSpace<EXACT, V> runs[kChainWaves], before[kChainWaves];
+    float state[64 * V];
     unsigned turn;
 };
 
 // State (gradient, when BACK) in front of wave w's span, from the span's own run and the value h in front of the whole sequence.
 // All waves of the workgroup call it; publishes what later batches wait for.
-template <bool BACK, int V>
-__device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned C, const Place &at, int order, int w, const Run (&own)[V],
+template <bool EXACT, bool BACK, int V>
+__device__ inline void chain_through(const Chain &ch, ChainSpace<EXACT, V> &m, unsigned C, const Place &at, int order, int w, const Run<EXACT> (&own)[V],
                                      float (&h)[V]) {
+    constexpr int kWords = Run<EXACT>::kWords;
     const int lane = (threadIdx.x & 63) * V, group = order / kGroup, rank = order - group * kGroup;
-#pragma unroll
-    for (int k = 0; k < V; k++) m.runs[w][0][lane + k] = own[k].A, m.runs[w][1][lane + k] = own[k].D, m.runs[w][2][lane + k] = own[k].B;
+    m.runs[w].put(own);
     __syncthreads();
     if (w == kChainWaves - 1 && rank < kGroup - 1 && order + 1 < ch.batches && at.mine) {
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            Run all = {1.f, 0.f, 0.f};
+            Run<EXACT> all = Run<EXACT>::none();
 #pragma unroll
             for (int i = 0; i < kChainWaves; i++) {
                 const int q = BACK ? kChainWaves - 1 - i : i;
-                all = run_join(all, Run{m.runs[q][0][lane + k], m.runs[q][1][lane + k], m.runs[q][2][lane + k]});
+                all = all.join(m.runs[q].get(k));
             }
-            float *o = ch.runs + (int64_t)order * 3 * C + at.c + k;
-            publish(o, all.A), publish(o + C, all.D), publish(o + 2 * (int64_t)C, all.B);
+            float *o = ch.runs + (int64_t)order * kWords * C + at.c + k;
+#pragma unroll
+            for (int q = 0; q < kWords; q++) publish(o + q * (int64_t)C, all.w[q]);
         }
     }
     const unsigned byte = at.c * 4u;                      // C < 2^30
     // the group's earlier batches, up to kEach to a wave
     constexpr int kEach = kGroup / kChainWaves;
     const int lo = w * kEach;
-    Run r[V];
+    Run<EXACT> r[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) r[k] = {1.f, 0.f, 0.f};
+    for (int k = 0; k < V; k++) r[k] = Run<EXACT>::none();
     if (lo < rank) {
-        unsigned bits[kEach][3][V];
+        unsigned bits[kEach][kWords][V];
         for (int tries = 0;; tries++) {
             bool ok = true;
 #pragma unroll
             for (int i = 0; i < kEach; i++)
 #pragma unroll
-                for (int q = 0; q < 3; q++)
+                for (int q = 0; q < kWords; q++)
 #pragma unroll
                     for (int k = 0; k < V; k++)
-                        bits[i][q][k] = lo + i < rank ? peek(ch.runs + ((int64_t)(group * kGroup + lo + i) * 3 + q) * C + k, byte) : 0u;
+                        bits[i][q][k] = lo + i < rank ? peek(ch.runs + ((int64_t)(group * kGroup + lo + i) * kWords + q) * C + k, byte) : 0u;
 #pragma unroll
             for (int i = 0; i < kEach; i++)
 #pragma unroll
-                for (int q = 0; q < 3; q++)
+                for (int q = 0; q < kWords; q++)
 #pragma unroll
                     for (int k = 0; k < V; k++) ok &= bits[i][q][k] != kEmpty;
             if (__all(ok) && ch.max_spins >= 0) break;
@@ -475,11 +519,14 @@ __device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned
         for (int i = 0; i < kEach; i++)
             if (lo + i < rank)
 #pragma unroll
-                for (int k = 0; k < V; k++)
-                    r[k] = run_join(r[k], Run{__uint_as_float(bits[i][0][k]), __uint_as_float(bits[i][1][k]), __uint_as_float(bits[i][2][k])});
-    }
+                for (int k = 0; k < V; k++) {
+                    Run<EXACT> then;
 #pragma unroll
-    for (int k = 0; k < V; k++) m.before[w][0][lane + k] = r[k].A, m.before[w][1][lane + k] = r[k].D, m.before[w][2][lane + k] = r[k].B;
+                    for (int q = 0; q < kWords; q++) then.w[q] = __uint_as_float(bits[i][q][k]);
+                    r[k] = r[k].join(then);
+                }
+    }
+    m.before[w].put(r);
     if (w == 0) {
         if (group > 0) {
             unsigned bits[V];
@@ -508,17 +555,17 @@ __device__ inline void chain_through(const Chain &ch, ChainSpace<V> &m, unsigned
     const int waves = (rank + kEach - 1) / kEach;
     for (int i = 0; i < waves; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = run_through(Run{m.before[i][0][lane + k], m.before[i][1][lane + k], m.before[i][2][lane + k]}, h[k]);
+        for (int k = 0; k < V; k++) h[k] = m.before[i].get(k).through(h[k]);
     const int steps = BACK ? kChainWaves - 1 - w : w;
     for (int i = 0; i < steps; i++) {
         const int q = BACK ? kChainWaves - 1 - i : i;
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = run_through(Run{m.runs[q][0][lane + k], m.runs[q][1][lane + k], m.runs[q][2][lane + k]}, h[k]);
+        for (int k = 0; k < V; k++) h[k] = m.runs[q].get(k).through(h[k]);
     }
     // the last batch of a group hands on the state behind it; the last wave in the chain's direction has it
     if (steps == kChainWaves - 1 && rank == kGroup - 1 && order + 1 < ch.batches && at.mine)
 #pragma unroll
-        for (int k = 0; k < V; k++) publish(ch.states + (int64_t)(group + 1) * C + at.c + k, run_through(own[k], h[k]));
+        for (int k = 0; k < V; k++) publish(ch.states + (int64_t)(group + 1) * C + at.c + k, own[k].through(h[k]));
 }
 
 // The batch that this workgroup draws: its tile's columns and wave w's span in it.
@@ -614,8 +661,8 @@ __global__ __launch_bounds__(64) void glr_forward_kernel(ForwardArgs<T> a) {
 // exchange their spans' runs through LDS.
 template <class T, int V>
 __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArgs<T> a) {
-    __shared__ float runs[kHeld][3][64 * V];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ RunSpace<sizeof(T) == 4, V> runs[kHeld];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Place at = place_of<V>(blockIdx.x, a.C, a.H, a.env_tiles);
     const int64_t t0 = (int64_t)w * kSpan;
     const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
@@ -627,24 +674,22 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
 #pragma unroll
     for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f;
     Span<V> g, u;
-    Run r[V];
+    Run<sizeof(T) == 4> r[V];
     span_open<T, V>(fr, xr, b, n, rm, g, u);
     span_run<sizeof(T) == 4, V>(g, u, rm, r);
+    runs[w].put(r);
 #pragma unroll
-    for (int k = 0; k < V; k++) {
-        runs[w][0][lane * V + k] = r[k].A, runs[w][1][lane * V + k] = r[k].D, runs[w][2][lane * V + k] = r[k].B;
-        h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
-    }
+    for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
     __syncthreads();
     for (int i = 0; i < w; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = run_through(Run{runs[i][0][lane * V + k], runs[i][1][lane * V + k], runs[i][2][lane * V + k]}, h[k]);
+        for (int k = 0; k < V; k++) h[k] = runs[i].get(k).through(h[k]);
     forward_span<T, V>(a, at, lane_offset(a.y, at), t0, n, rm, g, u, h);
 }
 
 template <class T, int V>
 __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_chain_kernel(ForwardArgs<T> a, Chain ch) {
-    __shared__ ChainSpace<V> mem;
+    __shared__ ChainSpace<sizeof(T) == 4, V> mem;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Drawn d = draw<false, V>(a, ch, mem.turn, w);
     Raw<T, V> fr, xr;
@@ -655,12 +700,12 @@ __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_
 #pragma unroll
     for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[d.at.j + k] : 0.f;
     Span<V> g, u;
-    Run r[V];
+    Run<sizeof(T) == 4> r[V];
     span_open<T, V>(fr, xr, b, d.n, rm, g, u);
     span_run<sizeof(T) == 4, V>(g, u, rm, r);
 #pragma unroll
     for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[d.at.c + k] : 0.f;
-    chain_through<false, V>(ch, mem, a.C, d.at, d.order, w, r, h);
+    chain_through<sizeof(T) == 4, false, V>(ch, mem, a.C, d.at, d.order, w, r, h);
     if (d.n > 0) forward_span<T, V>(a, d.at, lane_offset(a.y, d.at), d.t0, d.n, rm, g, u, h);
 }
 
@@ -827,9 +872,9 @@ __global__ __launch_bounds__(64, 2) void glr_backward_kernel(BackwardArgs<T> a) 
 
 template <class T>
 __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardArgs<T> a) {
-    __shared__ float runs[kHeld][3][64];
+    __shared__ RunSpace<sizeof(T) == 4, 1> runs[kHeld];
     __shared__ double sums[kHeld][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nw = blockDim.x >> 6;
     const Place at = place_of<1>(blockIdx.x, a.C, a.H, a.env_tiles);
     const int64_t t0 = (int64_t)w * kSpan;
     const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
@@ -842,19 +887,19 @@ __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardA
     float in[1] = {a.dh_last ? a.dh_last[at.c] : 0.f};
     double total[1] = {0.0};
     Span<1> g, q;
-    Run r[1];
+    Run<sizeof(T) == 4> r[1];
     back_open<T>(fr, xr, b, kept, n, rm, g, q);
     span_run_back<T>(g, gr, rm, r);
-    runs[w][0][lane] = r[0].A, runs[w][1][lane] = r[0].D, runs[w][2][lane] = r[0].B;
+    runs[w].put(r);
     __syncthreads();
-    for (int i = nw - 1; i > w; i--) in[0] = run_through(Run{runs[i][0][lane], runs[i][1][lane], runs[i][2][lane]}, in[0]);
+    for (int i = nw - 1; i > w; i--) in[0] = runs[i].get(0).through(in[0]);
     back_span<T>(a, at, lane_offset(a.df, at), lane_offset(a.dx, at), t0, n, rm, g, q, gr, in[0], total[0]);
     if (a.dbias_rows) dbias_row<kHeld>(a.dbias_rows, at, nw, total[0], sums);
 }
 
 template <class T>
 __global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel(BackwardArgs<T> a, Chain ch) {
-    __shared__ ChainSpace<1> mem;
+    __shared__ ChainSpace<sizeof(T) == 4, 1> mem;
     __shared__ double sums[kChainWaves][64];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Drawn d = draw<true, 1>(a, ch, mem.turn, w);
@@ -867,10 +912,10 @@ __global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel
     float in[1] = {a.dh_last ? a.dh_last[d.at.c] : 0.f};
     double total[1] = {0.0};
     Span<1> g, q;
-    Run r[1];
+    Run<sizeof(T) == 4> r[1];
     back_open<T>(fr, xr, b, kept, d.n, rm, g, q);
     span_run_back<T>(g, gr, rm, r);
-    chain_through<true, 1>(ch, mem, a.C, d.at, d.order, w, r, in);
+    chain_through<sizeof(T) == 4, true, 1>(ch, mem, a.C, d.at, d.order, w, r, in);
     if (d.n > 0) back_span<T>(a, d.at, lane_offset(a.df, d.at), lane_offset(a.dx, d.at), d.t0, d.n, rm, g, q, gr, in[0], total[0]);
     if (a.dbias_rows) dbias_row<kChainWaves>(a.dbias_rows + (int64_t)d.batch * a.C, d.at, kChainWaves, total[0], sums);
 }
@@ -972,7 +1017,7 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
 //   [512, E, H] bfloat16, 768 tiles: chain 75 / 140, walked 72 / 139; 1024: 97 / 185, 87 / 152; 4096: 365 / 718, 347 / 583
 struct Cut {
     enum { kHold, kWalk, kChain } how;
-    int V, env_tiles, batches;
+    int V, env_tiles, batches, words;        // words of a run
     int64_t tiles;
 };
 static Cut cut_of(int dtype, int T, int E, int H, bool back) {
@@ -985,6 +1030,7 @@ static Cut cut_of(int dtype, int T, int E, int H, bool back) {
     k.V = back ? 1 : wide;
     k.tiles = ceil_div(C, 64 * k.V);
     k.env_tiles = 0;
+    k.words = dtype == PPO2HIP_F32 ? Run<true>::kWords : Run<false>::kWords;
     k.batches = k.how == Cut::kChain ? (int)ceil_div(T, kBatch) : 1;
     return k;
 }
@@ -1010,12 +1056,12 @@ static int cut_check(const char *what, const Cut &k, int T, int64_t C) {
 }
 
 // words of a chain behind its counter
-static int64_t chain_words(const Cut &k, int64_t C) { return (3 * k.batches + ceil_div(k.batches, kGroup)) * C; }
+static int64_t chain_words(const Cut &k, int64_t C) { return ((int64_t)k.words * k.batches + ceil_div(k.batches, kGroup)) * C; }
 static size_t chain_bytes(const Cut &k, int64_t C) { return k.how == Cut::kChain ? 256 + align_up((size_t)chain_words(k, C) * sizeof(float), 256) : 0; }
 static int chain_begin(const Cut &k, int64_t C, void *workspace, Chain &ch, hipStream_t s) {
     ch.turn = (unsigned *)workspace;
     ch.runs = (float *)((char *)workspace + 256);
-    ch.states = ch.runs + 3 * k.batches * C;
+    ch.states = ch.runs + (int64_t)k.words * k.batches * C;
     ch.tiles = (unsigned)k.tiles;
     ch.batches = k.batches;
     // polls before a waiting wave gives up, about a second; PPO2HIP_GRID_SYNC_SPINS overrides it (negative: the first poll already counts as given up)
