@@ -424,7 +424,7 @@ struct RunSpace {
 // on who came first, so that results are the same bits every time.
 // A word is published by one agent-scope store and is its own flag: a launch before fills all words with kEmpty, a NaN that no
 // arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with NaN.
-constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan, kGroup = 32;
+constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan, kGroup = 16;
 constexpr unsigned kEmpty = 0xffffffffu;
 
 struct Chain {

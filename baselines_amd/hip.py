@@ -204,13 +204,13 @@ def _glr_apart(out, name, others):
 
 def _same_gpu(first, name, tensors):
     """Every tensor on the GPU of the first; True where that is not the current one."""
-    dev = first.device
-    if dev.type != "cuda":
+    gpu = first.get_device()
+    if not first.is_cuda:
         raise TypeError("%s must be a device tensor" % name)
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise TypeError("all tensors must be on %s" % dev)
-    return dev.index != torch.cuda.current_device()
+        if t is not None and t.get_device() != gpu:
+            raise TypeError("all tensors must be on %s" % first.device)
+    return gpu != torch._C._cuda_getDevice()
 
 
 class GlrSaved:
@@ -257,7 +257,7 @@ def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want
     st, se, _ = y.stride()
     check(lib.ppo2hip_glr_forward(code, T, E, H, sf, sx, pb, sr, p0, _lib.Seq(y.data_ptr(), st, se), h_last.data_ptr(),
                                   states.data_ptr() if want_saved else None, ws.data_ptr() if need else None, need,
-                                  _raw_stream(x.device.index)), "glr_forward")
+                                  _raw_stream(x.get_device())), "glr_forward")
     return y, h_last, GlrSaved(states, shape, dt) if want_saved else None
 
 
@@ -285,9 +285,9 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
         with torch.cuda.device(x.device):
             return glr_step(f, x, state, resets, bias, y)
     if y is None:
-        y = x.new_empty(shape)
-        sy = _lib.Seq(y.data_ptr(), 0, H)
-    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, sf, sx, pb, sr, ps, sy, ps, None, None, 0, _raw_stream(x.device.index)),
+        y = torch.empty_like(x)
+        sy = _lib.Seq(y.data_ptr(), 0, y.stride(0))
+    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, sf, sx, pb, sr, ps, sy, ps, None, None, 0, _raw_stream(x.get_device())),
           "glr_step")
     return y
 
@@ -342,7 +342,7 @@ def glr_backward(f, x, dy, saved, resets=None, bias=None, dh_last=None, df=None,
     xt, xe, _ = dx.stride()
     check(lib.ppo2hip_glr_backward(code, T, E, H, sf, sx, pb, sr, saved.states.data_ptr(), sdy, pl, _lib.Seq(df.data_ptr(), ft, fe),
                                    _lib.Seq(dx.data_ptr(), xt, xe), None if bias is None else dbias.data_ptr(), dh0.data_ptr(),
-                                   ws.data_ptr() if need else None, need, _raw_stream(x.device.index)), "glr_backward")
+                                   ws.data_ptr() if need else None, need, _raw_stream(x.get_device())), "glr_backward")
     return df, dx, dh0, dbias
 
 
