@@ -416,21 +416,27 @@ struct RunSpace {
 // ---------------------------------------------------------------------------------------------------------------------
 
 // Long sequences of few columns in one pass over the data: a workgroup holds kChainWaves spans of a tile in registers, a batch,
-// and the batches of a tile hand each other what they do to the state.  Workgroups draw batches from one counter, all tiles' first
-// ones before all second ones, so that whatever a batch waits for has been drawn by a workgroup that is running and that itself
-// only waits for earlier ones.  A batch
-// publishes its run; kGroup batches in a row form a group, whose last one publishes the state behind it instead.  A batch waits
-// for the runs of its group's earlier batches and for the state in front of the group: what is joined with what does not depend
-// on who came first, so that results are the same bits every time.
+// and the batches of a tile hand each other what they do to the state.  kChainWaves batches in a row form a group and as many groups a block.  A batch publishes its run, the
+// last one of a group the group's run, and the last one of a block the state behind it; a batch waits for the runs of its
+// group's earlier batches, one per wave, then for the runs of its block's earlier groups and the state in front of the block.
+// What is joined with what does not depend on who came first, so that results are the same bits every time.
 // A word is published by one agent-scope store and is its own flag: a launch before fills all words with kEmpty, a NaN that no
 // arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with NaN.
-constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan, kGroup = 16;
+//
+// Workgroups draw their seats, all tiles' first batches before all second ones, and wait for lower seats only.  Neighbouring tiles share
+// cache lines, and workgroups go to the XCDs in turn: each XCD's have a list of their own, eight seats in a row out of every 64,
+// behind a counter of its own; the seats behind the last 64 have a ninth.  The lowest seat that nobody has drawn is the next of its
+// list; whoever drew an earlier one of that list waits for drawn seats only and ends, and leaves room for the next workgroup of
+// that list.  [65536 x 1000 bfloat16] one counter 127 us (each draw of the 4096 takes 10 ns), lists 113.
+constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan;
 constexpr unsigned kEmpty = 0xffffffffu;
+constexpr int kTurnWords = 64, kTurnBytes = 9 * kTurnWords * sizeof(unsigned);
 
 struct Chain {
-    unsigned *turn;         // the counter, in 256 bytes of its own; then
+    unsigned *turn;         // counters, kTurnWords apart; behind them
     float *runs;            // [batches][words of a run][C]
-    float *states;          // [groups][C]: in front of groups 1, 2, ...
+    float *groups;          // [groups][words of a run][C]
+    float *states;          // [blocks][C]: in front of blocks 1, 2, ...
     unsigned tiles;
     int batches, max_spins;
     unsigned *fault;
@@ -447,7 +453,7 @@ __device__ inline unsigned peek(const float *base, unsigned c) {
 
 __global__ __launch_bounds__(256) void glr_chain_clear_kernel(Chain ch, int64_t words) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i == 0) *ch.turn = 0;
+    if (i < 4 * 9) ch.turn[i / 4 * kTurnWords] = 0;
     unsigned *p = (unsigned *)ch.runs + i;
     if (i + 4 <= words) *(uint4 *)p = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
     else
@@ -456,116 +462,119 @@ __global__ __launch_bounds__(256) void glr_chain_clear_kernel(Chain ch, int64_t 
 
 template <bool EXACT, int V>
 struct ChainSpace {
-    RunSpace<EXACT, V> runs[kChainWaves], before[kChainWaves];
+    RunSpace<EXACT, V> runs[kChainWaves], before[kChainWaves - 1], far[kChainWaves - 1];      // of spans, batches, groups
     float state[64 * V];
     unsigned turn;
 };
+
+// Waits until the lane's words at base [N][C], V of each, have been published.
+template <int N, int V>
+__device__ inline void await(const Chain &ch, const float *base, unsigned C, const Place &at, float (&v)[N][V]) {
+    const unsigned byte = at.c * 4u;                      // C < 2^30
+    unsigned bits[N][V];
+    for (int tries = 0;; tries++) {
+        bool ok = true;
+#pragma unroll
+        for (int q = 0; q < N; q++)
+#pragma unroll
+            for (int k = 0; k < V; k++) bits[q][k] = peek(base + q * (int64_t)C + k, byte);
+#pragma unroll
+        for (int q = 0; q < N; q++)
+#pragma unroll
+            for (int k = 0; k < V; k++) ok &= bits[q][k] != kEmpty;
+        if (__all(ok) && ch.max_spins >= 0) break;
+        if (tries >= ch.max_spins) {
+            if ((threadIdx.x & 63) == 0) atomicOr(ch.fault, kFaultGridSync);
+            break;
+        }
+        __builtin_amdgcn_s_sleep(1);
+    }
+#pragma unroll
+    for (int q = 0; q < N; q++)
+#pragma unroll
+        for (int k = 0; k < V; k++) v[q][k] = __uint_as_float(bits[q][k]);
+}
+template <bool EXACT, int V>
+__device__ inline void await_run(const Chain &ch, const float *runs, int64_t i, unsigned C, const Place &at, RunSpace<EXACT, V> &out) {
+    constexpr int kWords = Run<EXACT>::kWords;
+    float v[kWords][V];
+    await<kWords, V>(ch, runs + i * kWords * C, C, at, v);
+    Run<EXACT> r[V];
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int q = 0; q < kWords; q++) r[k].w[q] = v[q][k];
+    out.put(r);
+}
+template <bool EXACT, int V>
+__device__ inline void publish_run(float *runs, int64_t i, unsigned C, const Place &at, const Run<EXACT> (&r)[V]) {
+    constexpr int kWords = Run<EXACT>::kWords;
+    if (!at.mine) return;
+#pragma unroll
+    for (int k = 0; k < V; k++)
+#pragma unroll
+        for (int q = 0; q < kWords; q++) publish(runs + (i * kWords + q) * C + at.c + k, r[k].w[q]);
+}
 
 // State (gradient, when BACK) in front of wave w's span, from the span's own run and the value h in front of the whole sequence.
 // All waves of the workgroup call it; publishes what later batches wait for.
 template <bool EXACT, bool BACK, int V>
 __device__ inline void chain_through(const Chain &ch, ChainSpace<EXACT, V> &m, unsigned C, const Place &at, int order, int w, const Run<EXACT> (&own)[V],
                                      float (&h)[V]) {
-    constexpr int kWords = Run<EXACT>::kWords;
-    const int lane = (threadIdx.x & 63) * V, group = order / kGroup, rank = order - group * kGroup;
+    constexpr int kLast = kChainWaves - 1;
+    const int group = order / kChainWaves, rank = order % kChainWaves, block = group / kChainWaves, grank = group % kChainWaves;
+    const bool more = order + 1 < ch.batches;
+    Run<EXACT> all[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) all[k] = Run<EXACT>::none();
     m.runs[w].put(own);
     __syncthreads();
-    if (w == kChainWaves - 1 && rank < kGroup - 1 && order + 1 < ch.batches && at.mine) {
+    if (w < rank) {
+        await_run<EXACT, V>(ch, ch.runs, (int64_t)group * kChainWaves + w, C, at, m.before[w]);
+    } else if (w == kLast && more) {
+        for (int i = 0; i < kChainWaves; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) {
-            Run<EXACT> all = Run<EXACT>::none();
-#pragma unroll
-            for (int i = 0; i < kChainWaves; i++) {
-                const int q = BACK ? kChainWaves - 1 - i : i;
-                all = all.join(m.runs[q].get(k));
-            }
-            float *o = ch.runs + (int64_t)order * kWords * C + at.c + k;
-#pragma unroll
-            for (int q = 0; q < kWords; q++) publish(o + q * (int64_t)C, all.w[q]);
-        }
+            for (int k = 0; k < V; k++) all[k] = all[k].join(m.runs[BACK ? kLast - i : i].get(k));
+        if (rank < kLast) publish_run<EXACT, V>(ch.runs, order, C, at, all);
     }
-    const unsigned byte = at.c * 4u;                      // C < 2^30
-    // the group's earlier batches, up to kEach to a wave
-    constexpr int kEach = kGroup / kChainWaves;
-    const int lo = w * kEach;
-    Run<EXACT> r[V];
+    __syncthreads();
+    if (w < grank) {
+        await_run<EXACT, V>(ch, ch.groups, (int64_t)block * kChainWaves + w, C, at, m.far[w]);
+    } else if (w == kLast) {
+        if (rank == kLast && grank < kLast && more) {
+            Run<EXACT> whole[V];
 #pragma unroll
-    for (int k = 0; k < V; k++) r[k] = Run<EXACT>::none();
-    if (lo < rank) {
-        unsigned bits[kEach][kWords][V];
-        for (int tries = 0;; tries++) {
-            bool ok = true;
+            for (int k = 0; k < V; k++) whole[k] = Run<EXACT>::none();
+            for (int i = 0; i < kLast; i++)
 #pragma unroll
-            for (int i = 0; i < kEach; i++)
+                for (int k = 0; k < V; k++) whole[k] = whole[k].join(m.before[i].get(k));
 #pragma unroll
-                for (int q = 0; q < kWords; q++)
-#pragma unroll
-                    for (int k = 0; k < V; k++)
-                        bits[i][q][k] = lo + i < rank ? peek(ch.runs + ((int64_t)(group * kGroup + lo + i) * kWords + q) * C + k, byte) : 0u;
-#pragma unroll
-            for (int i = 0; i < kEach; i++)
-#pragma unroll
-                for (int q = 0; q < kWords; q++)
-#pragma unroll
-                    for (int k = 0; k < V; k++) ok &= bits[i][q][k] != kEmpty;
-            if (__all(ok) && ch.max_spins >= 0) break;
-            if (tries >= ch.max_spins) {
-                if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
-                break;
-            }
-            __builtin_amdgcn_s_sleep(1);
+            for (int k = 0; k < V; k++) whole[k] = whole[k].join(all[k]);
+            publish_run<EXACT, V>(ch.groups, group, C, at, whole);
         }
+        float v[1][V];
 #pragma unroll
-        for (int i = 0; i < kEach; i++)
-            if (lo + i < rank)
+        for (int k = 0; k < V; k++) v[0][k] = h[k];
+        if (block > 0) await<1, V>(ch, ch.states + (int64_t)block * C, C, at, v);
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    Run<EXACT> then;
-#pragma unroll
-                    for (int q = 0; q < kWords; q++) then.w[q] = __uint_as_float(bits[i][q][k]);
-                    r[k] = r[k].join(then);
-                }
-    }
-    m.before[w].put(r);
-    if (w == 0) {
-        if (group > 0) {
-            unsigned bits[V];
-            for (int tries = 0;; tries++) {
-                bool ok = true;
-#pragma unroll
-                for (int k = 0; k < V; k++) bits[k] = peek(ch.states + (int64_t)group * C + k, byte);
-#pragma unroll
-                for (int k = 0; k < V; k++) ok &= bits[k] != kEmpty;
-                if (__all(ok) && ch.max_spins >= 0) break;
-                if (tries >= ch.max_spins) {
-                    if (lane == 0) atomicOr(ch.fault, kFaultGridSync);
-                    break;
-                }
-                __builtin_amdgcn_s_sleep(1);
-            }
-#pragma unroll
-            for (int k = 0; k < V; k++) h[k] = __uint_as_float(bits[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < V; k++) m.state[lane + k] = h[k];
+        for (int k = 0; k < V; k++) m.state[(threadIdx.x & 63) * V + k] = v[0][k];
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < V; k++) h[k] = m.state[lane + k];
-    const int waves = (rank + kEach - 1) / kEach;
-    for (int i = 0; i < waves; i++)
+    for (int k = 0; k < V; k++) h[k] = m.state[(threadIdx.x & 63) * V + k];
+    for (int i = 0; i < grank; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = m.far[i].get(k).through(h[k]);
+    for (int i = 0; i < rank; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) h[k] = m.before[i].get(k).through(h[k]);
-    const int steps = BACK ? kChainWaves - 1 - w : w;
-    for (int i = 0; i < steps; i++) {
-        const int q = BACK ? kChainWaves - 1 - i : i;
+    const int steps = BACK ? kLast - w : w;
+    for (int i = 0; i < steps; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) h[k] = m.runs[q].get(k).through(h[k]);
-    }
-    // the last batch of a group hands on the state behind it; the last wave in the chain's direction has it
-    if (steps == kChainWaves - 1 && rank == kGroup - 1 && order + 1 < ch.batches && at.mine)
+        for (int k = 0; k < V; k++) h[k] = m.runs[BACK ? kLast - i : i].get(k).through(h[k]);
+    if (steps == kLast && rank == kLast && grank == kLast && more && at.mine)
 #pragma unroll
-        for (int k = 0; k < V; k++) publish(ch.states + (int64_t)(group + 1) * C + at.c + k, own[k].through(h[k]));
+        for (int k = 0; k < V; k++) publish(ch.states + (block + 1) * (int64_t)C + at.c + k, own[k].through(h[k]));
 }
 
 // The batch that this workgroup draws: its tile's columns and wave w's span in it.
@@ -576,9 +585,10 @@ struct Drawn {
 };
 template <bool BACK, int V, class Args>
 __device__ inline Drawn draw(const Args &a, const Chain &ch, unsigned &turn, int w) {
-    if (threadIdx.x == 0) turn = atomicAdd(ch.turn, 1u);
+    const unsigned whole = ch.tiles * (unsigned)ch.batches & ~63u, list = blockIdx.x < whole ? blockIdx.x & 7 : 8;
+    if (threadIdx.x == 0) turn = atomicAdd(ch.turn + list * kTurnWords, 1u);
     __syncthreads();
-    const unsigned u = __builtin_amdgcn_readfirstlane(turn);
+    const unsigned n = __builtin_amdgcn_readfirstlane(turn), u = list < 8 ? (n >> 3) * 64 + list * 8 + (n & 7) : whole + n;
     Drawn d;
     d.order = (int)(u / ch.tiles);
     d.batch = BACK ? ch.batches - 1 - d.order : d.order;
@@ -1055,13 +1065,17 @@ static int cut_check(const char *what, const Cut &k, int T, int64_t C) {
     return PPO2HIP_OK;
 }
 
-// words of a chain behind its counter
-static int64_t chain_words(const Cut &k, int64_t C) { return ((int64_t)k.words * k.batches + ceil_div(k.batches, kGroup)) * C; }
-static size_t chain_bytes(const Cut &k, int64_t C) { return k.how == Cut::kChain ? 256 + align_up((size_t)chain_words(k, C) * sizeof(float), 256) : 0; }
+// words of a chain behind its counters
+static int64_t chain_words(const Cut &k, int64_t C) {
+    const int64_t groups = ceil_div(k.batches, kChainWaves), blocks = ceil_div(groups, kChainWaves);
+    return (k.words * (k.batches + groups) + blocks) * C;
+}
+static size_t chain_bytes(const Cut &k, int64_t C) { return k.how == Cut::kChain ? kTurnBytes + align_up((size_t)chain_words(k, C) * sizeof(float), 256) : 0; }
 static int chain_begin(const Cut &k, int64_t C, void *workspace, Chain &ch, hipStream_t s) {
     ch.turn = (unsigned *)workspace;
-    ch.runs = (float *)((char *)workspace + 256);
-    ch.states = ch.runs + (int64_t)k.words * k.batches * C;
+    ch.runs = (float *)((char *)workspace + kTurnBytes);
+    ch.groups = ch.runs + (int64_t)k.words * k.batches * C;
+    ch.states = ch.groups + k.words * (int64_t)ceil_div(k.batches, kChainWaves) * C;
     ch.tiles = (unsigned)k.tiles;
     ch.batches = k.batches;
     // polls before a waiting wave gives up, about a second; PPO2HIP_GRID_SYNC_SPINS overrides it (negative: the first poll already counts as given up)
