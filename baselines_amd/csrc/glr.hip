@@ -415,7 +415,7 @@ struct RunSpace {
 // a chain of workgroups
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Long sequences of few columns in one pass over the data: a workgroup holds kChainWaves spans of a tile in registers, a batch,
+// Long sequences in one pass over the data: a workgroup holds kChainWaves spans of a tile in registers, a batch,
 // and the batches of a tile hand each other what they do to the state.  kChainWaves batches in a row form a group and as many groups a block.  A batch publishes its run, the
 // last one of a group the group's run, and the last one of a block the state behind it; a batch waits for the runs of its
 // group's earlier batches, one per wave, then for the runs of its block's earlier groups and the state in front of the block.
@@ -631,43 +631,7 @@ __device__ inline void forward_span(const ForwardArgs<T> &a, const Place &at, un
         for (int k = 0; k < V; k++) a.h_last[at.c + k] = h[k];
 }
 
-// A wave walks spans first .. end-1 of its columns from state h; the next span's inputs are on their way while a span is walked.
-template <class T, int V>
-__device__ inline void forward_walk(const ForwardArgs<T> &a, const Place &at, int64_t first, int64_t end, float (&h)[V]) {
-    const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at), yo = lane_offset(a.y, at);
-    float b[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[at.j + k] : 0.f;
-    Raw<T, V> fr, xr;
-    auto fetch = [&](int64_t s) {
-        const int64_t t0 = s * kSpan;
-        const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
-        fr.load(a.f, at, fo, t0, n);
-        xr.load(a.x, at, xo, t0, n);
-    };
-    if (first < end) fetch(first);
-    for (int64_t span = first; span < end; span++) {
-        const int64_t t0 = span * kSpan;
-        const int n = (int)(a.T_ - t0 < kSpan ? a.T_ - t0 : kSpan);
-        const unsigned rm = span_resets(a.resets, t0, n, at);
-        Span<V> g, u;
-        span_open<T, V>(fr, xr, b, n, rm, g, u);
-        if (span + 1 < end) fetch(span + 1);
-        forward_span<T, V>(a, at, yo, t0, n, rm, g, u, h);
-    }
-}
-
-// One wave per tile.
-template <class T, int V>
-__global__ __launch_bounds__(64) void glr_forward_kernel(ForwardArgs<T> a) {
-    const Place at = place_of<V>(blockIdx.x, a.C, a.H, a.env_tiles);
-    float h[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[at.c + k] : 0.f;
-    forward_walk<T, V>(a, at, 0, (a.T_ + kSpan - 1) / kSpan, h);
-}
-
-// Short sequences of few columns in one launch: a workgroup holds the whole of its columns, one span per wave, and the waves
+// Short sequences in one launch: a workgroup holds the whole of its columns, one span per wave, and the waves
 // exchange their spans' runs through LDS.
 template <class T, int V>
 __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArgs<T> a) {
@@ -736,7 +700,8 @@ struct BackwardArgs {
 
 // Gates and q = (p - x) a (1 - a), what df is per unit of g, from the states recomputed off the kept one.
 template <class T>
-__device__ inline void back_open(const Raw<T, 1> &f, const Raw<T, 1> &x, float b, float kept, int n, unsigned rm, Span<1> &g, Span<1> &q) {
+__device__ inline void back_open(const BackwardArgs<T> &a, const Place &at, const Raw<T, 1> &f, const Raw<T, 1> &x, float b, float kept, int64_t t0, int n,
+                                 unsigned rm, Span<1> &g, Span<1> &q) {
     typedef Gate<sizeof(T) == 4> G;
     constexpr bool kExact = sizeof(T) == 4;
     float h[1] = {kept}, slope;
@@ -758,14 +723,20 @@ __device__ inline void back_open(const Raw<T, 1> &f, const Raw<T, 1> &x, float b
         }
     }
     if (any_not_finite(h)) {
+        // the inputs once more from memory: kept for this, they would cost 32 registers
+        const char *fp = step_base(a.f, at, t0), *xp = step_base(a.x, at, t0);
+        const int64_t fstep = distance(a.f), xstep = distance(a.x);
+        const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at);
         h[0] = kept;
 #pragma unroll
-        for (int i = 0; i < kSpan; i++) {
-            const float xv = anew(x.get(i, 0)), v = G::of(anew(f.get(i, 0)) + b, slope);
-            if (anew(rm) >> i & 1) h[0] = 0.f;
-            g[i][0] = v;
-            q[i][0] = (h[0] - xv) * slope;
-            h[0] = G::pass_any(v, h[0]) + G::take(v) * xv;
+        for (int i = 0; i < kSpan; i++, fp += fstep, xp += xstep) {
+            if (i < n) {
+                const float xv = widen<T>(Raw<T, 1>::one(xp + here(xo))), v = G::of(widen<T>(Raw<T, 1>::one(fp + here(fo))) + b, slope);
+                if (anew(rm) >> i & 1) h[0] = 0.f;
+                g[i][0] = v;
+                q[i][0] = (h[0] - xv) * slope;
+                h[0] = G::pass_any(v, h[0]) + G::take(v) * xv;
+            }
         }
     }
     if (n < kSpan)
@@ -865,7 +836,7 @@ __device__ inline void backward_walk(const BackwardArgs<T> &a, const Place &at, 
         gr.load(a.dy, at, go, t0, n);
         const unsigned rm = span_resets(a.resets, t0, n, at);
         Span<1> g, q;
-        back_open<T>(fr, xr, b, kept, n, rm, g, q);
+        back_open<T>(a, at, fr, xr, b, kept, t0, n, rm, g, q);
         if (s > first) fetch(s - 1);
         back_span<T>(a, at, dfo, dxo, t0, n, rm, g, q, gr, in[0], total[0]);
     }
@@ -898,7 +869,7 @@ __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardA
     double total[1] = {0.0};
     Span<1> g, q;
     Run<sizeof(T) == 4> r[1];
-    back_open<T>(fr, xr, b, kept, n, rm, g, q);
+    back_open<T>(a, at, fr, xr, b, kept, t0, n, rm, g, q);
     span_run_back<T>(g, gr, rm, r);
     runs[w].put(r);
     __syncthreads();
@@ -923,7 +894,7 @@ __global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel
     double total[1] = {0.0};
     Span<1> g, q;
     Run<sizeof(T) == 4> r[1];
-    back_open<T>(fr, xr, b, kept, d.n, rm, g, q);
+    back_open<T>(a, d.at, fr, xr, b, kept, d.t0, d.n, rm, g, q);
     span_run_back<T>(g, gr, rm, r);
     chain_through<sizeof(T) == 4, true, 1>(ch, mem, a.C, d.at, d.order, w, r, in);
     if (d.n > 0) back_span<T>(a, d.at, lane_offset(a.df, d.at), lane_offset(a.dx, d.at), d.t0, d.n, rm, g, q, gr, in[0], total[0]);
@@ -987,7 +958,7 @@ __global__ void glr_copy_state_kernel(const float *src, float *dst, int64_t n) {
 
 using namespace ppo2hip;
 
-constexpr int64_t kWalkTiles = 896;       // tiles of a 16-bit sequence from which a wave walks all of its columns' steps
+constexpr int64_t kWalkTiles = 1280;      // tiles of a 16-bit sequence from which a wave walks back over all of its columns' steps
 
 template <class T>
 static Seq<T> seq_of(const ppo2hip_seq *s) {
@@ -1019,12 +990,13 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
     return ceil_div(T, kSpan) * (int64_t)E * H;
 }
 
-// How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile, walked by
-// one wave per tile, or passed along a chain of workgroups.  Measured, us forward / backward:
-//   [128, E, H] float32, 1024 tiles: held 20.9 / 38, walked 25.9 / 37.5; 4096 tiles: 84 / 141, 90 / 149
-//   [256, E, H] bfloat16, 512 tiles: held 26 / 47, walked 34 / 50; 1024: 49 / 95, 49 / 79; 4096: 180 / 385, 179 / 307
-//   [2048, E, H] float32, 384 tiles: chain 125 / 197, walked 226 / 491; 2048 tiles: 624 / 1056, 688 / 1127
-//   [512, E, H] bfloat16, 768 tiles: chain 75 / 140, walked 72 / 139; 1024: 97 / 185, 87 / 152; 4096: 365 / 718, 347 / 583
+// How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile (up to 256 steps),
+// passed along a chain of workgroups, or, back over many 16-bit columns, walked by one wave per tile, which has no exchange and keeps
+// 3 waves per SIMD loading.  Measured, us forward / backward:
+//   [128, 1024 x 64] float32: held 21 / 39, chain 26 / 41, walked 26 / 40; bfloat16 [128, 768 x 64]: 14 / 30, 20 / 35, 17 / 31
+//   [2048, 384 x 64] float32: chain 116 / 202, walked 233 / 375; 1024 x 64: 314 / 531, 330 / 539
+//   [2048, E, H] bfloat16, 768 x 64 columns: chain 122 / 264, walked 223 / 316; 1536 x 64: 240 / 512, 270 / 474; 4096 x 64: 641 / 1312,
+//   688 / 1290; [128, 1536 x 64]: held 18 / 37, walked 22 / 37; [256, 8192 x 64]: 165 / 354, 172 / 313
 struct Cut {
     enum { kHold, kWalk, kChain } how;
     int V, env_tiles, batches, words;        // words of a run
@@ -1034,8 +1006,8 @@ static Cut cut_of(int dtype, int T, int E, int H, bool back) {
     Cut k;
     const int64_t C = (int64_t)E * H;
     const int wide = dtype != PPO2HIP_F32 && H % 2 == 0 ? 2 : 1;
-    const bool many = dtype != PPO2HIP_F32 && ceil_div(C, 64 * wide) >= kWalkTiles, few = T <= kHeld * kSpan;
-    k.how = many && (back || !few) ? Cut::kWalk : few ? Cut::kHold : Cut::kChain;
+    const bool walk = back && dtype != PPO2HIP_F32 && ceil_div(C, 64) >= kWalkTiles;
+    k.how = walk ? Cut::kWalk : T <= kHeld * kSpan ? Cut::kHold : Cut::kChain;
     // two channels per lane halve a 16-bit sequence's loads and double what is in flight; going back there are no registers for them
     k.V = back ? 1 : wide;
     k.tiles = ceil_div(C, 64 * k.V);
@@ -1117,15 +1089,11 @@ static int forward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, 
         hipLaunchKernelGGL((glr_forward_held_kernel<T, V>), dim3((unsigned)k.tiles), dim3(threads_of(k, T_)), 0, s, a);
         return check_launch("glr_forward_held_kernel");
     }
-    if (k.how == Cut::kChain) {
-        Chain ch;
-        int rc = chain_begin(k, C, workspace, ch, s);
-        if (rc) return rc;
-        hipLaunchKernelGGL((glr_forward_chain_kernel<T, V>), dim3((unsigned)(k.tiles * k.batches)), dim3(64 * kChainWaves), 0, s, a, ch);
-        return check_launch("glr_forward_chain_kernel");
-    }
-    if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((glr_forward_kernel<T, V>), dim3((unsigned)k.tiles), dim3(64), 0, s, a);
-    return check_launch("glr_forward_kernel");
+    Chain ch;
+    int rc = chain_begin(k, C, workspace, ch, s);
+    if (rc) return rc;
+    hipLaunchKernelGGL((glr_forward_chain_kernel<T, V>), dim3((unsigned)(k.tiles * k.batches)), dim3(64 * kChainWaves), 0, s, a, ch);
+    return check_launch("glr_forward_chain_kernel");
 }
 
 extern "C" int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias,
