@@ -255,9 +255,9 @@ class MpiAdamW:
         self.t += 1
 
     def sync(self):
-        for p in self.plan.params:
-            self.comm.bcast_(p)
+        for p in self.params:
+            self.comm.bcast_(p.detach())
 
     def check_synced(self):
         if self.comm.size > 1:
-            self.comm.check_synced(torch.cat([p.reshape(-1).float() for p in self.plan.params]))
+            self.comm.check_synced(torch.cat([p.detach().reshape(-1).float() for p in self.params]))

@@ -642,8 +642,8 @@ def take_faults(raise_on_fault=True):
 def fault_error(bits):
     """The exception a non-zero fault word stands for."""
     if bits & FAULT_GRID_SYNC:
-        return _lib.Ppo2HipError("a launch whose workgroups hand values to each other (whole-sequence LSTM, or the optimiser step folded "
-                                 "into the epoch call) gave up waiting for its peers (is the GPU shared with another job?); results since "
+        return _lib.Ppo2HipError("a launch whose workgroups hand values to each other (whole-sequence LSTM, the optimiser step folded "
+                                 "into the epoch call, or a long gated linear recurrence) gave up waiting for its peers (is the GPU shared with another job?); results since "
                                  "the last check are invalid — PPO2HIP_LSTM_SEQ_OFF=1 takes one LSTM launch per step")
     what = [name for bit, name in ((FAULT_INDEX_RANGE, "a minibatch index list"), (FAULT_COMPOSE_RANGE, "a permutation handed to compose"))
             if bits & bit]
@@ -1005,7 +1005,7 @@ class AdamWPlan:
             if not p.is_cuda or p.device != dev:
                 raise TypeError("params[%d] must be a tensor of the first one's GPU" % k)
         self.device, self.state_bits = dev, state_bits
-        self.params = [p.detach() for p in params]
+        self.params = params
         self.grad_dtypes = [grad_dtype or p.dtype for p in params]
         self._ptrs = [p.data_ptr() for p in params]
         self._numels = [p.numel() for p in params]
@@ -1034,6 +1034,9 @@ class AdamWPlan:
                 if state_bits == 8 and t.data_ptr() % 4:
                     raise ValueError("state %s must be aligned to 4 bytes" % name)
                 setattr(self, name, t)
+            spans = sorted(spans + [_extent(t) for t in state if t.numel()])
+            if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+                raise ValueError("state overlaps itself or params")
             image = np.zeros(int(lib.ppo2hip_adamw_plan_bytes(self._tensors, n)), np.uint8)
             check(lib.ppo2hip_adamw_plan_fill(self._tensors, n, state_bits, image.ctypes.data_as(ctypes.c_void_p), image.size),
                   "adamw_plan_fill")
@@ -1051,9 +1054,9 @@ class AdamWPlan:
             raise ValueError("adamw_step needs one gradient (or None) per tensor: %d for %d" % (len(grads), len(self._ptrs)))
         gpu = self.device.index
         for g, dt, n in zip(grads, self.grad_dtypes, self._numels):
-            if g is not None and not (g.dtype is dt and g.get_device() == gpu and g.numel() == n and g.is_contiguous()):
+            if g is not None and not (isinstance(g, torch.Tensor) and g.dtype is dt and g.get_device() == gpu and g.numel() == n and g.is_contiguous()):
                 k = next(i for i, h in enumerate(grads) if h is g)
-                if g.dtype is not dt or g.get_device() != gpu:
+                if not isinstance(g, torch.Tensor) or g.dtype is not dt or g.get_device() != gpu:
                     raise TypeError("grads[%d] must be %s on %s" % (k, dt, self.device))
                 raise ValueError("grads[%d] must be contiguous with %d entries" % (k, n))
         if [p.data_ptr() for p in self.params] != self._ptrs:
@@ -1066,7 +1069,9 @@ def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_
     """One AdamW step of every tensor of ``plan``: step count ``t`` (1 for the first), gradients in list order (contiguous; None
     leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by the norm over all of them when
     ``max_grad_norm`` > 0.  Bias-corrected roots next to ``epsilon`` and decay apart from the gradient: unlike :func:`adam_step`,
-    which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  A HIP graph that captures the call keeps ``lr`` and ``t``."""
+    which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  Gradients must not share memory with the parameters or moments.  A
+    plan's steps go one after the other, also those of HIP graphs that captured them (they share its moments and workspace); a
+    captured call keeps ``lr``, ``t`` and the gradients' addresses."""
     if plan.device.index != torch.cuda.current_device():
         with torch.cuda.device(plan.device):
             return adamw_step(plan, grads, lr, t, beta1, beta2, epsilon, weight_decay, max_grad_norm, grad_scale)

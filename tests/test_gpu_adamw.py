@@ -430,3 +430,23 @@ def test_small_and_large_epsilons(hip, sizes, eps, scale):
         (new, nm, nv, gs), _, _ = reference(old, grads, m, v, lr, t, [0] * len(sizes), wd=0.0, eps=eps)
         for k in range(len(sizes)):
             close(ps[k], new[k], tol_p(old[k], new[k], lr, m[k], nm[k], nv[k], t, gs[k]), ("p", k, t))
+
+
+def test_what_a_plan_refuses_to_share(hip):
+    """Moments in one place with each other or with a parameter, a parameter whose storage was exchanged behind the plan, and gradients
+    that are no tensors."""
+    z = lambda n, dt=F32: torch.zeros(n, dtype=dt, device="cuda")      # noqa: E731
+    p, both = z(300), z(700)
+    for state in ((both[:300], both[200:500]), (both[:300], both[:300]), (p, z(300))):
+        with pytest.raises(ValueError, match="overlaps"):
+            hip.AdamWPlan([p], state=state)
+    plan = hip.AdamWPlan([p], state=(both[:300], both[300:600]))
+    with pytest.raises(TypeError):
+        hip.adamw_step(plan, [3.0], 0.1, 1)
+    layer = torch.nn.Linear(3, 2, device="cuda")
+    plan = hip.AdamWPlan(layer.parameters())
+    grads = [torch.ones_like(q) for q in plan.params]
+    hip.adamw_step(plan, grads, 0.1, 1)
+    layer.weight.data = layer.weight.data.clone()
+    with pytest.raises(ValueError, match="moved"):
+        hip.adamw_step(plan, grads, 0.1, 2)
