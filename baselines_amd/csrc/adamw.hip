@@ -18,7 +18,7 @@ constexpr int kMaxGrads = 448;                   // gradient pointers of one lau
 constexpr int kNormGroups = 4096;                // most workgroups of the norm launch, each with a partial sum
 constexpr int kOwnSums = 512;                    // most partial sums that every workgroup of the step adds up by itself
 constexpr int kOwnChunks = 2048;                 // chunks from which it does not
-constexpr int kSmallThreads = 1024, kSmallChunks = kSmallThreads / 64;   // chunks up to which every workgroup of the step sums all squares itself
+constexpr int kSmallThreads = 1024, kSmallChunks = 32;   // chunks up to which every workgroup of the step sums all squares itself
 
 struct TensorRow {                               // one tensor in the device image of a plan
     void *p;
@@ -214,8 +214,9 @@ __device__ inline float over_root(float m, float v, float eps) {
 }
 
 // THREADS kThreads: a workgroup per chunk.  kSmallThreads, for lists of at most kSmallChunks chunks that are clipped: the same,
-// after each of its waves has summed the squares of one of the list's chunks, so that the norm needs no launch of its own.
-// [13 tensors, 11 k parameters] 3.7 + 6.5 us in two launches, 7.7 in one, and the host queues one less (3.4 us).
+// after its waves have summed the squares of the whole list, so that the norm needs no launch of its own.  In one launch / in two, us
+// per replay and per eager call, 32-bit moments: 8 chunks 5.1 and 9.5 / -, 24 chunks 6.5 and 9.0 / 7.1 and 12.2, 32 chunks 7.9 and
+// 9.0 / 7.2 and 12.5, 64 chunks 11.5 and 11.7 / 7.2 and 12.6; 8-bit, 32 chunks: 8.7 and 9.3 / 9.3 and 12.3.
 template <int BITS, int THREADS>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a) {
     constexpr int kParts = (kChunk + 4 * THREADS - 1) / (4 * THREADS);
@@ -255,8 +256,9 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a) {
         if (a.max_norm > 0.f) {
             float norm;
             if (THREADS == kSmallThreads) {
-                const int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-                norm = (float)sqrt(block_sum(c < a.nchunks ? chunk_squares<64>(a, c, threadIdx.x & 63) : 0.0, red));
+                double sum = 0.0;
+                for (int c = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < a.nchunks; c += THREADS / 64) sum += chunk_squares<64>(a, c, threadIdx.x & 63);
+                norm = (float)sqrt(block_sum(sum, red));
             } else {
                 norm = norm_of(a.partial, a.npartial, red);
             }
