@@ -197,7 +197,8 @@ int ppo2hip_compose_i32(const int32_t *prev, const int32_t *sigma, int32_t *out,
 #define PPO2HIP_FAULT_INDEX_RANGE 1u
 #define PPO2HIP_FAULT_COMPOSE_RANGE 2u
 #define PPO2HIP_FAULT_GRID_SYNC 4u      /* a launch whose workgroups hand values to each other (whole-sequence LSTM, the
-                                         * optimiser step folded into ppo2hip_ppo_epoch) gave up waiting for its peers */
+                                         * optimiser step folded into ppo2hip_ppo_epoch, a gated linear recurrence of more
+                                         * than 256 steps) gave up waiting for its peers */
 int ppo2hip_take_faults(uint32_t *bits, void *stream);
 /* The same read-and-clear queued on `stream` WITHOUT waiting: a one-thread kernel stores the word into *host_bits
  * (page-locked HOST memory the device can address, e.g. from hipHostMalloc, that stays valid until the kernel has run;
@@ -497,8 +498,11 @@ typedef struct ppo2hip_seq {
  *   h0 : float32 [E, H] or NULL (zeros)        h_last : float32 [E, H] out or NULL; may be h0 itself when T = 1
  *   saved : float32 [ppo2hip_glr_saved_floats(T, E, H)] out or NULL: the states in front of steps 0, SPAN, 2 SPAN, ...,
  *           which ppo2hip_glr_backward recomputes the others from
- *   workspace : ppo2hip_glr_forward_workspace_bytes(...) bytes (may be 0)
- * E*H may reach 2^31 - 1.  T = 0 copies h0 to h_last. */
+ *   workspace : ppo2hip_glr_forward_workspace_bytes(...) bytes (may be 0), 16-byte aligned, for this call alone until it has run;
+ *               nothing is kept in it from call to call
+ * E*H may reach 2^31 - 1 and H 2^26 - 1 (more than 256 steps: E*H below 2^30).  T = 0 copies h0 to h_last.
+ * Up to 256 steps one launch; more: a small launch that clears the workspace and one whose workgroups hand the state on.  Their waits
+ * are bounded: one that gives up raises PPO2HIP_FAULT_GRID_SYNC (ppo2hip_take_faults) and leaves NaN behind. */
 int64_t ppo2hip_glr_saved_floats(int T, int E, int H);
 size_t ppo2hip_glr_forward_workspace_bytes(int dtype, int T, int E, int H);
 int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias,
@@ -519,8 +523,10 @@ int ppo2hip_glr_backward(int dtype, int T, int E, int H, const ppo2hip_seq *f, c
  * AdamW over many tensors
  * ---------------------------------------------------------------------- */
 
-/* One step of Adam with decoupled weight decay over a list of tensors, in one launch (two when clipping); a list of more
- * than 448 tensors takes as many again per further 448.  Beside ppo2hip_adam_step (one flat float32 arena, epsilon next to the uncorrected root, no decay) it has
+/* One step of Adam with decoupled weight decay over a list of tensors, in one launch; clipped, lists of up to 32 chunks of 2048
+ * elements (each tensor its own) still take one, up to 2048 chunks two, longer ones three.  A list of more than 448 tensors takes
+ * as many again per further 448.  Beside ppo2hip_adam_step (one flat float32 arena, epsilon next to the uncorrected root, no decay)
+ * it has
  *   g = grad * grad_scale, times max_grad_norm / max(norm, max_grad_norm) over ALL tensors' norm when max_grad_norm > 0
  *   m = beta1 m + (1 - beta1) g     v = beta2 v + (1 - beta2) g^2
  *   p -= lr (m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon) + weight_decay * decay * p)
@@ -549,7 +555,9 @@ size_t ppo2hip_adamw_workspace_bytes(const ppo2hip_adamw_tensor *tensors, int nt
 /*   tensors : HOST, as the plan was filled from     plan : DEVICE image     grads : HOST array of DEVICE pointers or NULLs
  *   m, v : DEVICE moments (float32, or int8 / uint8 codes)     m_scale, v_scale : DEVICE float32, 8 bits only
  *   norm_out : DEVICE float[2] or NULL: {norm of grad * grad_scale (written when clipping), factor applied to grads}
- *   workspace : DEVICE, ppo2hip_adamw_workspace_bytes bytes, only used when clipping
+ *   workspace : DEVICE, ppo2hip_adamw_workspace_bytes bytes, 16-byte aligned, only used when clipping
+ * Gradients must not share memory with parameters or moments.  Steps of one list go one after the other: they share its moments
+ * (and workspace), also where HIP graphs captured them.
  * All host arguments are read before the call returns; a HIP graph that captures the call keeps their values. */
 int ppo2hip_adamw_step(const ppo2hip_adamw_tensor *tensors, int ntensors, int state_bits, const void *plan,
                        const void *const *grads, void *m, float *m_scale, void *v, float *v_scale, double lr, int64_t t,
