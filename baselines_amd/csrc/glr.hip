@@ -427,15 +427,15 @@ struct RunSpace {
 // A word is published by one agent-scope store and is its own flag: a launch before fills all words with kEmpty, a NaN that no
 // arithmetic makes.  Every wait is bounded; a wave that gives up raises the library's fault word and carries on with NaN.
 //
-// Workgroups draw their seats, all tiles' first batches before all second ones, and wait for lower seats only.  As in seat_of, each
-// XCD's workgroups have a list of their own, eight seats in a row out of every 64, behind a counter of its own; the seats behind
-// the last 64 have a ninth.  The lowest seat that nobody has drawn is the next of its list; whoever drew an earlier one of that
-// list waits for drawn seats only, so it ends and leaves room for the next workgroup of that list.  (Dealt to the XCDs in another
-// way, but started in order, the lists advance together, and fewer than 64 workgroups wait for a seat that is not drawn.)
-// One counter for all: 127 us for [65536, 1, 1000] bfloat16, each of its 4096 draws takes 10 ns; the lists: 113.
+// Four tiles in a row share a counter, behind which their batches are given out in order, all four tiles' first ones before the second
+// ones: what a batch waits for, earlier batches of its own tile, has been drawn by workgroups that are running and that wait for still
+// earlier ones only, whatever else runs on the card and wherever workgroups start.  One counter for all tiles is drawn from once in
+// 10 ns: [2048, 16, 512] float32 50 us, a counter per four tiles 43, per tile 44 and [16384, 4, 1024] bfloat16 95, 97, 100 (tiles
+// that drift apart in time share no cache lines).  Lists of seats per XCD were 113 us for [65536, 1, 1000] bfloat16 where this takes
+// 125, but a workgroup then waits for seats that no running one has drawn, which two such launches at once can turn into a deadlock.
 constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan;
 constexpr unsigned kEmpty = 0xffffffffu;
-constexpr int kTurnWords = 64, kTurnBytes = 9 * kTurnWords * sizeof(unsigned);
+constexpr int kTurnWords = 64, kTurns = 64, kTurnTiles = 4, kTurnBytes = kTurns * kTurnWords * sizeof(unsigned);
 
 struct Chain {
     unsigned *turn;         // counters, kTurnWords apart; behind them
@@ -458,7 +458,7 @@ __device__ inline unsigned peek(const float *base, unsigned c) {
 
 __global__ __launch_bounds__(256) void glr_chain_clear_kernel(Chain ch, int64_t words) {
     const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i < 4 * 9) ch.turn[i / 4 * kTurnWords] = 0;
+    if (i < 4 * kTurns) ch.turn[i / 4 * kTurnWords] = 0;
     unsigned *p = (unsigned *)ch.runs + i;
     if (i + 4 <= words) *(uint4 *)p = make_uint4(kEmpty, kEmpty, kEmpty, kEmpty);
     else
@@ -590,14 +590,16 @@ struct Drawn {
 };
 template <bool BACK, int V, class Args>
 __device__ inline Drawn draw(const Args &a, const Chain &ch, unsigned &turn, int w) {
-    const unsigned whole = ch.tiles * (unsigned)ch.batches & ~63u, list = blockIdx.x < whole ? blockIdx.x & 7 : 8;
-    if (threadIdx.x == 0) turn = atomicAdd(ch.turn + list * kTurnWords, 1u);
+    // counter c serves the tiles of groups c, c + kTurns, ...; as many workgroups draw from it as it has seats
+    const unsigned groups = (ch.tiles + kTurnTiles - 1) / kTurnTiles, c = seat_of(blockIdx.x) % ch.tiles / kTurnTiles % kTurns;
+    const unsigned last = c + (groups - 1 - c) / kTurns * kTurns, share = (last - c) / kTurns * kTurnTiles + min(ch.tiles - last * kTurnTiles, (unsigned)kTurnTiles);
+    if (threadIdx.x == 0) turn = atomicAdd(ch.turn + c * kTurnWords, 1u);
     __syncthreads();
-    const unsigned n = __builtin_amdgcn_readfirstlane(turn), u = list < 8 ? (n >> 3) * 64 + list * 8 + (n & 7) : whole + n;
+    const unsigned n = __builtin_amdgcn_readfirstlane(turn), i = n % share;
     Drawn d;
-    d.order = (int)(u / ch.tiles);
+    d.order = (int)(n / share);
     d.batch = BACK ? ch.batches - 1 - d.order : d.order;
-    d.at = place_of<V>(u - (unsigned)d.order * ch.tiles, a.C, a.H, a.env_tiles);
+    d.at = place_of<V>((c + i / kTurnTiles * kTurns) * kTurnTiles + i % kTurnTiles, a.C, a.H, a.env_tiles);
     d.t0 = ((int64_t)d.batch * kChainWaves + w) * kSpan;
     d.n = (int)(a.T_ - d.t0 < kSpan ? a.T_ - d.t0 : kSpan);
     return d;
@@ -667,8 +669,9 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
 }
 
 // Bound by what of the loads and the hand-over the 16 waves of a CU do not hide from each other: of 12 us that a workgroup lives, 3.2
-// are loads, 1.2 the draw, 0.5 the gates, 5 waits.  [65536, 1, 1000] bfloat16, 393 MB: 108 us (3.6 TB/s; a copy in the same tiles 76),
-// [16384, 4, 1024]: 94.  Two channels per lane: one 123 and 99 us.  Waves of a workgroup: 4, 16: 151, 112 where 8 took 107.
+// are loads, 1.2 the draw, 0.5 the gates, 5 waits.  bfloat16 [65536, 1, 1000], 393 MB: 122 us (3.2 TB/s; a copy in the same tiles 102: rows
+// of 2000 bytes, whose lines neighbouring tiles fetch twice), [65536, 1, 1024] 106, [16384, 4, 1024] 96.  Two channels per lane:
+// with one 11 and 5 us more.  Waves of a workgroup: 4, 16: 151, 112 us where 8 took 107.
 template <class T, int V>
 __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_chain_kernel(ForwardArgs<T> a, Chain ch) {
     __shared__ ChainSpace<sizeof(T) == 4, V> mem;

@@ -456,3 +456,27 @@ def test_bias_gradient_over_many_rows(hip, T, E, H):
     """More rows of partial sums than one workgroup adds up, and columns that end inside a workgroup's 32."""
     a, normal = make(T, E, H, F32, bias=True, seed=E)
     check(hip, a, normal, F32)
+
+
+def test_several_calls_at_once(hip):
+    """Chains of workgroups on four streams at a time: each hands on its own states and none waits for another."""
+    sizes = [(9000, 2, 130), (4000, 3, 257), (20000, 1, 96), (2100, 8, 200)]
+    calls = []
+    for i, (T, E, H) in enumerate(sizes):
+        a, normal = make(T, E, H, (F32, BF16)[i % 2], resets=True, bias=True, seed=i)
+        calls.append((a, normal(T, E, H).to(a["x"].dtype), torch.cuda.Stream()))
+
+    def both(a, dy):
+        y, last, saved = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+        return (y, last) + hip.glr_backward(a["f"], a["x"], dy, saved, resets=a["resets"], bias=a["bias"])
+    want = [both(a, dy) for a, dy, _ in calls]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for a, dy, s in calls:
+            with torch.cuda.stream(s):
+                got.append(both(a, dy))
+    torch.cuda.synchronize()
+    hip.take_faults()
+    for k, outs in enumerate(got):
+        assert all(torch.equal(p, q) for p, q in zip(outs, want[k % len(calls)])), k
