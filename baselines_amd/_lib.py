@@ -144,6 +144,7 @@ _SIGS = {
     "ppo2hip_glr_forward": (c_int, [c_int, c_int, c_int, c_int, POINTER(Seq), POINTER(Seq), _P, POINTER(Seq), _P, POINTER(Seq), _P,
                                     _P, _P, c_size_t, _P]),
     "ppo2hip_glr_backward_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
+    "ppo2hip_glr_step": (c_int, [c_int, c_int, c_int, _P, c_int64, _P, c_int64, _P, _P, c_int64, _P, _P, c_int64, _P]),
     "ppo2hip_glr_backward": (c_int, [c_int, c_int, c_int, c_int, POINTER(Seq), POINTER(Seq), _P, POINTER(Seq), _P, POINTER(Seq), _P,
                                      POINTER(Seq), POINTER(Seq), _P, _P, _P, c_size_t, _P]),
     "ppo2hip_adamw_state_elements": (c_int64, [POINTER(AdamwTensor), c_int, c_int]),

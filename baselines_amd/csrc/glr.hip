@@ -1141,6 +1141,13 @@ extern "C" int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip
 #undef PPO2HIP_GLR_FORWARD
 }
 
+extern "C" int ppo2hip_glr_step(int dtype, int E, int H, const void *f, int64_t f_e, const void *x, int64_t x_e, const float *bias,
+                                const uint8_t *resets, int64_t resets_e, float *state, void *y, int64_t y_e, void *stream) {
+    PPO2HIP_REQUIRE(state || (int64_t)E * H == 0, "glr_step: state is null");
+    const ppo2hip_seq fs = {(void *)f, 0, f_e}, xs = {(void *)x, 0, x_e}, ys = {y, 0, y_e}, rs = {(void *)resets, 0, resets_e};
+    return ppo2hip_glr_forward(dtype, 1, E, H, &fs, &xs, bias, resets ? &rs : nullptr, state, &ys, state, nullptr, nullptr, 0, stream);
+}
+
 template <class T>
 static int backward_of(const Cut &k, const ppo2hip_seq *f, const ppo2hip_seq *x, const float *bias, const ppo2hip_seq *resets, const float *saved,
                        const ppo2hip_seq *dy, const float *dh_last, const ppo2hip_seq *df, const ppo2hip_seq *dx, float *dbias, float *dh0,

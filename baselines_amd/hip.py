@@ -230,7 +230,8 @@ def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want
     projection, batch-first tensors); ``resets`` [T, E] flags set BEFORE step t, as the rollout's dones are; ``bias`` [H]
     and ``h0`` [E, H] float32 (default zeros).  Returns (y, h_last, saved): y in x's type, the last state [E, H] in float32 and,
     with ``want_saved``, what :func:`glr_backward` needs.  ``y`` and ``h_last`` may be brought; they must not overlap each
-    other or the inputs."""
+    other or the inputs.  Beyond 256 steps workgroups hand the state to each other; should one ever give up waiting, :func:`take_faults`
+    says so."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _GLR_TYPES:
         raise TypeError("x must be a float32, bfloat16 or float16 tensor [T, E, H]")
     shape, dt = x.shape, x.dtype
@@ -268,8 +269,8 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
         raise TypeError("x must be a float32, bfloat16 or float16 tensor [E, H]")
     shape, dt = x.shape, x.dtype
     E, H = shape
-    sf, sx = _glr_row(f, "f", shape, dt), _glr_row(x, "x", shape, dt)
-    pb, ps, sr = _glr_f32(bias, "bias", (H,)), _glr_f32(state, "state", shape), None
+    fe, xe = _glr_row(f, "f", shape, dt), _glr_row(x, "x", shape, dt)
+    pb, ps, pr, re = _glr_f32(bias, "bias", (H,)), _glr_f32(state, "state", shape), None, 0
     if state is None:
         raise TypeError("state must be a float32 tensor")
     if resets is not None:
@@ -277,31 +278,31 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
             raise TypeError("resets must be a bool or uint8 tensor")
         if resets.shape != (E,):
             raise ValueError("resets must have shape %s, got %s" % ((E,), tuple(resets.shape)))
-        sr = _lib.Seq(resets.data_ptr(), 0, resets.stride(0))
+        pr, re = resets.data_ptr(), resets.stride(0)
     if y is not None:
-        sy = _glr_row(y, "y", shape, dt)
+        ye = _glr_row(y, "y", shape, dt)
         _glr_apart(y.unsqueeze(0), "y", (("f", f.unsqueeze(0)), ("x", x.unsqueeze(0)), ("state", state), ("resets", resets), ("bias", bias)))
     if _same_gpu(x, "x", (f, bias, resets, state, y)):
         with torch.cuda.device(x.device):
             return glr_step(f, x, state, resets, bias, y)
     if y is None:
         y = torch.empty_like(x)
-        sy = _lib.Seq(y.data_ptr(), 0, y.stride(0))
-    check(lib.ppo2hip_glr_forward(_GLR_TYPES[dt], 1, E, H, sf, sx, pb, sr, ps, sy, ps, None, None, 0, _raw_stream(x.get_device())),
-          "glr_step")
+        ye = y.stride(0)
+    check(lib.ppo2hip_glr_step(_GLR_TYPES[dt], E, H, f.data_ptr(), fe, x.data_ptr(), xe, pb, pr, re, ps, y.data_ptr(), ye,
+                               _raw_stream(x.get_device())), "glr_step")
     return y
 
 
 def _glr_row(t, name, shape, dtype):
-    """[E, H] tensor with a contiguous last dimension, as one step of a sequence."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+    """The stride over E of an [E, H] tensor with a contiguous last dimension."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype:
         raise TypeError("%s must be a %s tensor" % (name, dtype))
     if t.shape != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
     se, sj = t.stride()
     if sj != 1 and shape[1] > 1:
         raise ValueError("%s must be contiguous over its last dimension" % name)
-    return _lib.Seq(t.data_ptr(), 0, se)
+    return se
 
 
 def glr_backward(f, x, dy, saved, resets=None, bias=None, dh_last=None, df=None, dx=None):

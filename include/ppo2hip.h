@@ -509,6 +509,11 @@ int ppo2hip_glr_forward(int dtype, int T, int E, int H, const ppo2hip_seq *f, co
                         const ppo2hip_seq *resets, const float *h0, const ppo2hip_seq *y, float *h_last, float *saved,
                         void *workspace, size_t workspace_bytes, void *stream);
 
+/* One acting step, state [E, H] float32 advanced in place: ppo2hip_glr_forward with T = 1 and h0 = h_last = state, for callers to
+ * whom a call's microseconds matter.  The int64 behind f, x, resets (or NULL) and y are their strides over envs in elements. */
+int ppo2hip_glr_step(int dtype, int E, int H, const void *f, int64_t f_e, const void *x, int64_t x_e, const float *bias,
+                     const uint8_t *resets, int64_t resets_e, float *state, void *y, int64_t y_e, void *stream);
+
 /* Gradients of the same layer from dy and dh_last (float32 [E, H] or NULL: zeros); f, x, bias, resets and saved as the
  * forward call had and left them.
  *   df, dx : dtype [T, E, H] out      dbias : float32 [H] out or NULL, summed over t and e in a fixed order

@@ -196,3 +196,13 @@ def test_c_entry_refuses_lists_and_norms_that_do_not_fit(_lib):
     for clip in (1e-60, float("nan")):
         assert step(clip) == _lib.EINVAL and b"max_grad_norm" in L.ppo2hip_last_error()
     assert step(1.0, ws=ctypes.c_void_p(264)) == _lib.EINVAL and step(1.0, plan=ctypes.c_void_p(264)) == _lib.EINVAL
+
+
+def test_c_entry_refuses_bad_steps(_lib):
+    L, one = _lib.lib, ctypes.c_void_p(256)
+    step = lambda dt=0, E=3, H=8, f=one, fe=8, x=one, r=None, re=1, s=one, y=one: L.ppo2hip_glr_step(      # noqa: E731
+        dt, E, H, f, fe, x, 8, None, r, re, s, y, 8, None)
+    for kw in (dict(dt=3), dict(E=-1), dict(H=-1), dict(H=1 << 26), dict(f=None), dict(x=None), dict(y=None), dict(s=None), dict(fe=-8),
+               dict(r=one, re=-1)):
+        assert step(**kw) == _lib.EINVAL and L.ppo2hip_last_error(), kw
+    assert step(E=0, s=None) == 0 and step(H=0) == 0
