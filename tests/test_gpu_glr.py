@@ -480,3 +480,13 @@ def test_several_calls_at_once(hip):
     hip.take_faults()
     for k, outs in enumerate(got):
         assert all(torch.equal(p, q) for p, q in zip(outs, want[k % len(calls)])), k
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_16_bit_sequences(hip, dtype):
+    """Over several blocks of batches, 128 * 64 steps each, with a reset now and then in one env only."""
+    T, E, H = 17000, 2, 66
+    a, normal = make(T, E, H, dtype, bias=True, seed=5)
+    a["resets"] = torch.zeros(T, E, dtype=torch.bool, device="cuda")
+    a["resets"][[0, 8191, 8192, 16390], 1] = True
+    check(hip, a, normal, dtype)
