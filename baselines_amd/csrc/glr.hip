@@ -22,19 +22,17 @@ constexpr int kHeld = 16;                                   // spans that a work
 // gates
 // ---------------------------------------------------------------------------------------------------------------------
 
-// How a step's gate is held between the passes over a span, by the sequence's type.
-//   16 bits: om = 1 - a itself.  a v is v - om v: off by 2^-25 of v at most, which shows in 16 bits only where a single step shrinks
-//   the state by 2^13 and more.  The rounding of the exponent and of the reciprocal stay.
-//   float32: the smaller side s = min(a, 1 - a) <= 1/2, negated where that is 1 - a (a >= 1/2, by the sign bit, -0 included): both
-//   sides keep their relative accuracy, and what the exponent's product and the reciprocal round is made good.
-// Either way 1 - a is never taken from a rounded a: it would lose the memory's length as soon as a is near one.
-// slope: a (1 - a), the gate's derivative.
+// How a step's gate is held between the passes over a span: the smaller side s = min(a, 1 - a) <= 1/2, negated where that is 1 - a
+// (a >= 1/2, by the sign bit, -0 included), so that both sides keep their relative accuracy.  1 - a from a rounded a would lose the
+// memory's length as soon as a is near one, and a from a rounded 1 - a what is left of a large state behind a gate near zero.
+// For float32 sequences what the exponent's product and the reciprocal round is made good; 16 bits keep it (|z| 2^-24 and two ulp).
 template <bool EXACT>
-struct Gate;
-
-template <>
-struct Gate<true> {
+struct Gate {
     static __device__ inline float of(float z) {
+        if (!EXACT) {
+            const float e = __builtin_amdgcn_exp2f(fabsf(z) * -1.44269502f), s = e * __builtin_amdgcn_rcpf(1.f + e);
+            return z >= 0.f ? -s : s;                       // a NaN is one on both sides
+        }
         float m = fabsf(z);
         m = m > 128.f ? 128.f : m;                          // e^-128 is 0 in float32; a NaN stays one
         const float t = m * -1.44269502f;
@@ -46,7 +44,7 @@ struct Gate<true> {
         r = fmaf(fmaf(-d, r, 1.f), r, r);
         return copysignf(e * r, -z);
     }
-    static __device__ inline float of(float z, float &slope) {
+    static __device__ inline float of(float z, float &slope) {                                       // a (1 - a), the gate's derivative
         const float v = of(z);
         slope = fabsf(v) * (1.f - fabsf(v));
         return v;
@@ -59,21 +57,6 @@ struct Gate<true> {
     }
     static __device__ inline float open() { return -0.f; }  // a = 1
     static __device__ inline float shut() { return 0.f; }   // a = 0
-};
-
-template <>
-struct Gate<false> {
-    static __device__ inline float of(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * 1.44269502f)); }
-    static __device__ inline float of(float z, float &slope) {
-        const float e = __builtin_amdgcn_exp2f(fabsf(z) * -1.44269502f), r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
-        slope = s * r;                                      // from the smaller side: 1 - om has no figures left where a is small
-        return z >= 0.f ? s : r;                            // a NaN is one on both sides
-    }
-    static __device__ inline float take(float v) { return v; }
-    static __device__ inline float pass(float v, float h) { return fmaf(-v, h, h); }
-    static __device__ inline float pass_any(float v, float h) { return fabsf(h) < INFINITY ? pass(v, h) : (1.f - v) * h; }
-    static __device__ inline float open() { return 0.f; }
-    static __device__ inline float shut() { return 1.f; }
 };
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -113,7 +96,7 @@ struct Run<false> {
     float w[2];
     static __device__ inline float live(float A) { return fmaxf(A, 0x1p-149f); }
     static __device__ inline Run none() { return {{1.f, 0.f}}; }
-    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? 0.f : live(D <= 0.5f ? 1.f - D : A), 0.f}}; }
+    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? 0.f : live(A > 0.5f ? 1.f - D : A), 0.f}}; }
     __device__ inline void add(float B) { w[1] = B; }
     __device__ inline float through(float h) const { return w[0] == 0.f ? w[1] : fmaf(w[0], h, w[1]); }
     __device__ inline Run join(const Run &r) const { return {{r.w[0] == 0.f || w[0] == 0.f ? 0.f : live(w[0] * r.w[0]), r.through(w[1])}}; }
@@ -346,7 +329,8 @@ __device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm
     }
 }
 
-// What a span lets through.  D = 1 - A grows by 1 - a of what is left of it, so that it keeps its figures while it is small.
+// What a span lets through.  D = 1 - A grows by 1 - a of what is left of it, so that it keeps its figures while it is small.  For 16
+// bits D counts only where A ends above 1/2, which no gate below 1/2 leaves it: there 1 - a is the gate as it is held, negated.
 template <bool EXACT, int V>
 __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run<EXACT> (&r)[V]) {
     typedef Gate<EXACT> G;
@@ -357,7 +341,7 @@ __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run<EXACT> (&r
     for (int i = 0; i < kSpan; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) {
-            const float om = G::take(g[i][k]);
+            const float om = EXACT ? G::take(g[i][k]) : -g[i][k];
             A[k] = G::pass(g[i][k], A[k]);
             D[k] = D[k] + fmaf(-D[k], om, om);
         }

@@ -490,3 +490,42 @@ def test_long_16_bit_sequences(hip, dtype):
     a["resets"] = torch.zeros(T, E, dtype=torch.bool, device="cuda")
     a["resets"][[0, 8191, 8192, 16390], 1] = True
     check(hip, a, normal, dtype)
+
+
+def _relative(share, each, back=False):
+    """Relative error of a scan whose terms are all positive, step by step: what came over by its share of the step's value, and
+    `each` for the step itself."""
+    r, out = torch.zeros_like(share[0]), torch.empty_like(share)
+    for t in range(share.shape[0] - 1, -1, -1) if back else range(share.shape[0]):
+        r = share[t] * r + each
+        out[t] = r
+    return out
+
+
+@pytest.mark.parametrize("T", [1, 5, 40, 300, 9000])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gates_almost_shut_keep_their_share(hip, T, dtype):
+    """States of 1e4 behind gates of 1e-8 beside inputs of 1e-3, and gradients likewise.  Every term is positive, so errors stay
+    relative: a gate's (8 + 2 Z) U, two products, the sum, and three roundings where runs are joined, twice that for good measure."""
+    E, H, z = 2, 70, 18.375
+    g = torch.Generator(device="cuda").manual_seed(T)
+    kind = torch.rand((T, E, H), generator=g, device="cuda")
+    f = torch.where(kind < 0.6, -z, torch.where(kind < 0.8, 0.0, 3.0)).to(dtype)
+    x = (torch.where((kind >= 0.6) & (kind < 0.8), 1e4, 1e-3) * (0.5 + torch.rand((T, E, H), generator=g, device="cuda"))).to(dtype)
+    h0 = 1e4 * (0.5 + torch.rand((E, H), generator=g, device="cuda"))
+    y, last, saved = hip.glr_forward(f, x, h0, want_saved=True)
+    want, wlast, ps = ref.forward(f, x, h0)
+    each = (20 + 2 * z) * ref.U
+    a = torch.sigmoid(f.double())
+    rel = _relative(a * ps / want, each)
+    close(y, want, rel * want, "y")
+    close(last, wlast, rel[-1] * wlast, "h_last")
+    kind = torch.rand((T, E, H), generator=g, device="cuda")
+    dy = (torch.where(kind < 0.3, 1e4, 1e-3) * (0.5 + torch.rand((T, E, H), generator=g, device="cuda"))).to(dtype)
+    dl = 1e4 * (0.5 + torch.rand((E, H), generator=g, device="cuda"))
+    _, dx, dh0, _ = hip.glr_backward(f, x, dy, saved, dh_last=dl)
+    _, wx, w0, _ = ref.backward(f, x, h0, None, None, dy, dl)
+    om = torch.sigmoid(-f.double())
+    rel = _relative(1 - dy.double() * om / wx, each, back=True)
+    close(dx, wx, (rel + each) * wx, "dx")
+    close(dh0, w0, (rel[0] + each) * w0, "dh0")
