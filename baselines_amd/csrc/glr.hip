@@ -52,9 +52,8 @@ struct Gate {
     static __device__ inline bool keeps(float v) { return (int)__float_as_uint(v) < 0; }
     static __device__ inline float take(float v) { return keeps(v) ? -v : 1.f - v; }                 // 1 - a
     static __device__ inline float pass(float v, float h) { return fmaf(v, h, keeps(v) ? h : 0.f); } // a h
-    static __device__ inline float pass_any(float v, float h) {                                     // where h may not be finite
-        return fabsf(h) < INFINITY ? pass(v, h) : (keeps(v) ? 1.f + v : v) * h;
-    }
+    // where h may not be finite: an infinite state passes every gate, however little of it is open, as it passes a run of gates
+    static __device__ inline float pass_any(float v, float h) { return fabsf(h) < INFINITY ? pass(v, h) : v + h; }
     static __device__ inline float open() { return -0.f; }  // a = 1
     static __device__ inline float shut() { return 0.f; }   // a = 0
 };

@@ -480,8 +480,8 @@ int ppo2hip_ppo_epoch_shares(const ppo2hip_policy_desc *desc, const ppo2hip_loss
  * in the reference; its masks are those of the reference's LSTM (a flag set BEFORE step t empties the state,
  * baselines/a2c/utils.py:86-147).  Per env e and channel j:
  *   a[t] = sigmoid(f[t] + bias)     p[t] = resets[t] ? 0 : h[t-1]     h[t] = a[t] p[t] + (1 - a[t]) x[t]     y[t] = h[t]
- * A state that a reset empties has no influence on what follows, infinities and NaN included.  The state, both scans, the
- * sums and everything between loads and stores are float32. */
+ * A state that a reset empties has no influence on what follows, infinities and NaN included; an infinite one passes every
+ * gate, also one of f + bias = -infinity.  The state, both scans, the sums and everything between loads and stores are float32. */
 enum { PPO2HIP_F32 = 0, PPO2HIP_BF16 = 1, PPO2HIP_F16 = 2 };
 #define PPO2HIP_GLR_SPAN 16    /* steps between two kept states */
 

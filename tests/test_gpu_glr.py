@@ -529,3 +529,72 @@ def test_gates_almost_shut_keep_their_share(hip, T, dtype):
     rel = _relative(1 - dy.double() * om / wx, each, back=True)
     close(dx, wx, (rel + each) * wx, "dx")
     close(dh0, w0, (rel[0] + each) * w0, "dh0")
+
+
+
+_FAR = [-17.0, -30.0, -60.0, -88.0, -100.0, -110.0, -300.0, -700.0, 17.0, 60.0, 86.0, 0.5, 88.0, 110.0, 300.0, 700.0]
+
+
+@pytest.mark.parametrize("T", [1, 5, 40, 600, 9000])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_infinite_states_pass_every_gate(hip, T, dtype):
+    """sigmoid of a finite number is not zero: an infinite state, input or gradient stays one however far the gate, in the span that
+    it enters and in all that follow.  The definition makes it no number at a gate of minus infinity, and 1 - a of a gate beyond 87 is
+    zero in the hardware's exponent: what is left there is not finite either way."""
+    H = len(_FAR)
+    f = torch.tensor(_FAR, device="cuda").to(dtype).expand(T, 4, H).contiguous()
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x, dy = ((0.5 + torch.rand((T, 4, H), generator=g, device="cuda")).to(dtype) for _ in range(2))
+    h0 = 0.5 + torch.rand(4, H, generator=g, device="cuda")
+    h0[0] = float("inf")                            # env 0 begins so, env 1 meets an infinity on the way, env 2 a shut gate behind one
+    x[T // 3, 1, :12] = -float("inf")
+    h0[2] = -float("inf")
+    f[T // 2, 2] = -float("inf")
+    dl = torch.ones(4, H, device="cuda")
+    dl[0] = float("inf")
+    dy[(2 * T) // 3, 1] = float("inf")
+    y, last, saved = hip.glr_forward(f, x, h0, want_saved=True)
+    want, wlast, _ = ref.forward(f, x, h0)
+    df, dx, dh0, _ = hip.glr_backward(f, x, dy, saved, dh_last=dl)
+    _, wx, w0, _ = ref.backward(f, x, h0, None, None, dy, dl)
+    for name, got, w in (("y", y, want), ("h_last", last, wlast), ("dx", dx, wx), ("dh0", dh0, w0)):
+        assert torch.equal(torch.isfinite(got), torch.isfinite(w)), name
+        sure = torch.isinf(w)                       # infinite by the definition
+        if name == "dx":
+            sure[:, :, 12:] = False
+        assert torch.equal(got[sure].double(), w[sure]), name
+        fin = torch.isfinite(w)
+        # at most T steps of (20 + 2 Z) U of values of at most 3/2 (g: at most T of them and the last), and half a step of the type
+        top = 1.5 if name in ("y", "h_last") else 1.5 * T + 1
+        tol = (20 + 2 * 700) * T * ref.U * top + half_step(got.dtype) * w[fin].abs()
+        assert bool(((got[fin].double() - w[fin]).abs() <= tol).all()), name
+
+
+@pytest.mark.parametrize("T", [5, 40, 700, 9000])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("E,H", [(2, 70), (3, 33)])
+def test_what_a_reset_hides_in_16_bits(hip, T, dtype, E, H):
+    """What is not finite stays in its own column, and in front of the reset, bit for bit, in both directions."""
+    r = T // 2
+    a, normal = make(T, E, H, dtype, bias=True)
+    a["resets"] = torch.zeros(T, E, dtype=torch.uint8, device="cuda")
+    a["resets"][r] = 1
+    dy = normal(T, E, H).to(dtype)
+    clean = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    gclean = hip.glr_backward(a["f"], a["x"], dy, clean[2], resets=a["resets"], bias=a["bias"])
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        h0, x = a["h0"].clone(), a["x"].clone()
+        h0[0, 3] = bad
+        x[r - 1, 1, 5] = bad
+        y, last, saved = hip.glr_forward(a["f"], x, h0, resets=a["resets"], bias=a["bias"], want_saved=True)
+        assert torch.equal(y[r:], clean[0][r:]) and torch.equal(last, clean[1])
+        assert not bool(torch.isfinite(y[:r, 0, 3]).any()) and not bool(torch.isfinite(y[r - 1, 1, 5]))
+        rest = torch.ones_like(y, dtype=torch.bool)
+        rest[:r, 0, 3] = False
+        rest[r - 1, 1, 5] = False
+        assert torch.equal(y[rest], clean[0][rest])
+        dyb = dy.clone()
+        dyb[r, 1, 9] = bad
+        df, dx, dh0, _ = hip.glr_backward(a["f"], x, dyb, saved, resets=a["resets"], bias=a["bias"])
+        assert torch.equal(dx[:r], gclean[1][:r]) and torch.equal(dh0, gclean[2])
+        assert torch.equal(df[r + 1:], gclean[0][r + 1:])
