@@ -348,7 +348,7 @@ __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run<EXACT> (&r
     for (int k = 0; k < V; k++) r[k] = Run<EXACT>::of(A[k], D[k], rm != 0);
 }
 
-// A span's run in the direction of time,
+// A span's run in the direction of time.
 template <bool EXACT, int V>
 __device__ inline void span_run(const Span<V> &g, const Span<V> &u, unsigned rm, Run<EXACT> (&r)[V]) {
     float h[V];
@@ -359,7 +359,73 @@ __device__ inline void span_run(const Span<V> &g, const Span<V> &u, unsigned rm,
 #pragma unroll
     for (int k = 0; k < V; k++) r[k].add(h[k]);
 }
-// and against it, for the gradient: dy enters a step before the gate does, a reset stands behind it.
+
+// The same for a chain in 16 bits, which leaves in g and u what the steps up to each let through of the state in front of the span and
+// the state that they build up from zero, so that the outputs are one product and sum each once that state is known.  What a step
+// lets through is off by 2^-25 for each step before it, which 16 bits do not show; the state behind the span goes by D.
+// [65536, 1, 1000] bfloat16: 131 us with a walk in either place, 127 so; where a workgroup holds the sequence the walk is quicker
+// ([128, 512, 256]: 24.5, 27).
+template <class T, int V, bool WHOLE>
+__device__ inline void scan_steps(const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int n, unsigned rm, Span<V> &g, Span<V> &u, float (&D)[V]) {
+    typedef Gate<false> G;
+    float A[V], h[V];
+#pragma unroll
+    for (int k = 0; k < V; k++) A[k] = 1.f, D[k] = h[k] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSpan; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            float v = G::of(f.get(i, k) + b[k]), add = G::take(v) * x.get(i, k);
+            if (!WHOLE) {
+                if (i >= n) v = G::open(), add = 0.f;
+                v = with_reset<false>(v, rm, i);
+            }
+            A[k] = G::pass(v, A[k]);
+            D[k] = D[k] + fmaf(-D[k], -v, -v);              // as in span_passes
+            h[k] = G::pass(v, h[k]) + add;
+            g[i][k] = A[k];
+            u[i][k] = h[k];
+        }
+}
+template <class T, int V, class Args>
+__device__ inline void span_scan(const Args &a, const Place &at, const Raw<T, V> &f, const Raw<T, V> &x, const float (&b)[V], int64_t t0, int n, unsigned rm,
+                                 Span<V> &g, Span<V> &u, Run<false> (&r)[V]) {
+    typedef Gate<false> G;
+    float D[V];
+    if (n >= kSpan && !__any(rm != 0)) scan_steps<T, V, true>(f, x, b, n, rm, g, u, D);
+    else scan_steps<T, V, false>(f, x, b, n, rm, g, u, D);
+    if (any_not_finite(u[kSpan - 1])) {
+        // the inputs once more from memory: kept for this, they would cost 32 registers
+        asm volatile("" : "+s"(t0));
+        const char *fp = step_base(a.f, at, t0), *xp = step_base(a.x, at, t0);
+        const int64_t fstep = distance(a.f), xstep = distance(a.x);
+        const unsigned fo = lane_offset(a.f, at), xo = lane_offset(a.x, at);
+        Raw<T, V> in;
+        float h[V];
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kSpan; i++, fp += fstep, xp += xstep) {
+            if (i < n) {
+                in.v[0] = in.one(fp + here(fo)), in.v[1] = in.one(xp + here(xo));
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    const float v = G::of(in.get(0, k) + b[k]), add = G::take(v) * in.get(1, k);
+                    h[k] = anew(rm) >> i & 1 ? add : G::pass_any(v, h[k]) + add;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < V; k++) u[i][k] = h[k];
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < V; k++) {
+        r[k] = Run<false>::of(g[kSpan - 1][k], D[k], rm != 0);
+        r[k].add(u[kSpan - 1][k]);
+    }
+}
+
+// A span's run against time, for the gradient: dy enters a step before the gate does, a reset stands behind it.
 template <class T>
 __device__ inline void span_run_back(const Span<1> &g, const Raw<T, 1> &dy, unsigned rm, Run<sizeof(T) == 4> (&r)[1]) {
     typedef Gate<sizeof(T) == 4> G;
@@ -603,19 +669,48 @@ struct ForwardArgs {
     unsigned C, H, env_tiles;
 };
 
-template <class T, int V>
+template <class T, int V, bool SCAN>
 __device__ inline void forward_span(const ForwardArgs<T> &a, const Place &at, unsigned yo, int64_t t0, int n, unsigned rm, const Span<V> &g,
-                                    const Span<V> &u, float (&h)[V]) {
+                                    const Span<V> &u, const Run<sizeof(T) == 4> (&r)[V], float (&h)[V]) {
     if (!at.mine) return;
     if (a.saved)
 #pragma unroll
         for (int k = 0; k < V; k++) a.saved[t0 / kSpan * a.C + at.c + k] = h[k];
     char *p = nullptr;
     const int64_t step = distance(a.y);
-    span_walk<sizeof(T) == 4, V>(g, u, rm, n >= kSpan, n, h, [&](int i, const float (&v)[V]) {
+    auto put = [&](int i, const float (&v)[V]) {
         p = i == 0 ? step_base(a.y, at, t0) : p + step;
         Lane<T, V>::store(p + here(yo), v);
-    });
+    };
+    if constexpr (!SCAN) {
+        span_walk<sizeof(T) == 4, V>(g, u, rm, n >= kSpan, n, h, put);
+    } else {
+        float v[V];
+        if (n >= kSpan && !any_not_finite(h)) {
+#pragma unroll
+            for (int i = 0; i < kSpan; i++) {
+#pragma unroll
+                for (int k = 0; k < V; k++) {
+                    v[k] = fmaf(g[i][k], h[k], u[i][k]);
+                    asm("" : "+v"(v[k]));                   // float32 first: fused with its rounding to 16 bits it is not the slow way's
+                }
+                put(i, v);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kSpan; i++)
+                if (i < n) {
+#pragma unroll
+                    for (int k = 0; k < V; k++) {
+                        v[k] = fabsf(h[k]) < INFINITY ? fmaf(g[i][k], h[k], u[i][k]) : h[k] + u[i][k];
+                        if (anew(rm) << (31 - i)) v[k] = u[i][k];           // a reset at step i or before
+                    }
+                    put(i, v);
+                }
+        }
+#pragma unroll
+        for (int k = 0; k < V; k++) h[k] = r[k].through(h[k]);
+    }
     if (a.h_last && t0 + kSpan >= a.T_)
 #pragma unroll
         for (int k = 0; k < V; k++) a.h_last[at.c + k] = h[k];
@@ -648,7 +743,7 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
     for (int i = 0; i < w; i++)
 #pragma unroll
         for (int k = 0; k < V; k++) h[k] = runs[i].get(k).through(h[k]);
-    forward_span<T, V>(a, at, lane_offset(a.y, at), t0, n, rm, g, u, h);
+    forward_span<T, V, false>(a, at, lane_offset(a.y, at), t0, n, rm, g, u, r, h);
 }
 
 // Bound by what of the loads and the hand-over the 16 waves of a CU do not hide from each other: of 12 us that a workgroup lives, 3.2
@@ -669,12 +764,16 @@ __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_
     for (int k = 0; k < V; k++) b[k] = a.bias ? a.bias[d.at.j + k] : 0.f;
     Span<V> g, u;
     Run<sizeof(T) == 4> r[V];
-    span_open<T, V>(fr, xr, b, d.n, rm, g, u);
-    span_run<sizeof(T) == 4, V>(g, u, rm, r);
+    if constexpr (sizeof(T) == 4) {
+        span_open<T, V>(fr, xr, b, d.n, rm, g, u);
+        span_run<true, V>(g, u, rm, r);
+    } else {
+        span_scan<T, V>(a, d.at, fr, xr, b, d.t0, d.n, rm, g, u, r);
+    }
 #pragma unroll
     for (int k = 0; k < V; k++) h[k] = a.h0 ? a.h0[d.at.c + k] : 0.f;
     chain_through<sizeof(T) == 4, false, V>(ch, mem, a.C, d.at, d.order, w, r, h);
-    if (d.n > 0) forward_span<T, V>(a, d.at, lane_offset(a.y, d.at), d.t0, d.n, rm, g, u, h);
+    if (d.n > 0) forward_span<T, V, sizeof(T) == 2>(a, d.at, lane_offset(a.y, d.at), d.t0, d.n, rm, g, u, r, h);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
