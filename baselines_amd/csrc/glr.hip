@@ -539,6 +539,10 @@ __device__ inline void await(const Chain &ch, const float *base, unsigned C, con
         if (__all(ok) && ch.max_spins >= 0) break;
         if (tries >= ch.max_spins) {
             if ((threadIdx.x & 63) == 0) atomicOr(ch.fault, kFaultGridSync);
+#pragma unroll
+            for (int q = 0; q < N; q++)
+#pragma unroll
+                for (int k = 0; k < V; k++) bits[q][k] = kEmpty;    // NaN as a whole: some words may have come
             break;
         }
         __builtin_amdgcn_s_sleep(1);

@@ -598,3 +598,34 @@ def test_what_a_reset_hides_in_16_bits(hip, T, dtype, E, H):
         df, dx, dh0, _ = hip.glr_backward(a["f"], x, dyb, saved, resets=a["resets"], bias=a["bias"])
         assert torch.equal(dx[:r], gclean[1][:r]) and torch.equal(dh0, gclean[2])
         assert torch.equal(df[r + 1:], gclean[0][r + 1:])
+
+
+_GAVE_UP_VALUES_SCRIPT = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch
+from baselines_amd import hip
+for dt in (torch.float32, torch.bfloat16):
+    T, E, H = 700, 2, 70
+    f, x, dy = (torch.randn(T, E, H, device="cuda").to(dt) for _ in range(3))
+    y, last, saved = hip.glr_forward(f, x, want_saved=True)
+    df, dx, dh0, _ = hip.glr_backward(f, x, dy, saved)
+    hip.take_faults(raise_on_fault=False)
+    ok = bool(torch.isfinite(y[:128]).all()) and bool(torch.isnan(y[128:]).all()) and bool(torch.isnan(last).all())
+    ok = ok and bool(torch.isfinite(dx[640:]).all()) and bool(torch.isnan(dx[:640]).all()) and bool(torch.isnan(dh0).all())
+    print("VALUES", ok)
+"""
+
+
+def test_a_chain_that_gave_up_leaves_nan(tmp_path):
+    """Behind the batch of 128 steps that waits for nobody nothing looks like a result, whatever had been published by then."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    script = tmp_path / "gave_up.py"
+    script.write_text(_GAVE_UP_VALUES_SCRIPT)
+    env = dict(os.environ, PPO2HIP_GRID_SYNC_SPINS="-1")
+    res = subprocess.run([sys.executable, str(script), root], env=env, capture_output=True, text=True, timeout=100)
+    assert res.returncode == 0, res.stderr[-2000:]
+    assert [l for l in res.stdout.splitlines() if l.startswith("VALUES")] == ["VALUES True"] * 2, res.stdout
