@@ -264,7 +264,7 @@ def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want
 
 def glr_step(f, x, state, resets=None, bias=None, y=None):
     """One acting step of :func:`glr_forward` for E envs: ``f``, ``x`` [E, H], ``resets`` [E]; ``state`` [E, H] float32 is advanced
-    in place.  Returns y [E, H] in x's type."""
+    in place and overlaps none of the others.  Returns y [E, H] in x's type."""
     if not isinstance(x, torch.Tensor) or x.dim() != 2 or x.dtype not in _GLR_TYPES:
         raise TypeError("x must be a float32, bfloat16 or float16 tensor [E, H]")
     shape, dt = x.shape, x.dtype
@@ -279,6 +279,12 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
         if resets.shape != (E,):
             raise ValueError("resets must have shape %s, got %s" % ((E,), tuple(resets.shape)))
         pr, re = resets.data_ptr(), resets.stride(0)
+    pf, px, es, end = f.data_ptr(), x.data_ptr(), 4 if dt is torch.float32 else 2, ps + 4 * E * H
+    if (pf < end and ps < pf + ((E - 1) * fe + H) * es or px < end and ps < px + ((E - 1) * xe + H) * es or
+            pb and pb < end and ps < pb + 4 * H or pr and pr < end and ps <= pr + (E - 1) * re):
+        for name, p, n, step, width in (("f", pf, E, fe * es, H * es), ("x", px, E, xe * es, H * es), ("bias", pb, 1, 0, 4 * H), ("resets", pr, E, re, 1)):
+            if p and ps < end and _rows_meet(ps, end, p, n, step, width):
+                raise ValueError("state overlaps %s" % name)
     if y is not None:
         ye = _glr_row(y, "y", shape, dt)
         _glr_apart(y.unsqueeze(0), "y", (("f", f.unsqueeze(0)), ("x", x.unsqueeze(0)), ("state", state), ("resets", resets), ("bias", bias)))
@@ -288,9 +294,15 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
     if y is None:
         y = torch.empty_like(x)
         ye = y.stride(0)
-    check(lib.ppo2hip_glr_step(_GLR_TYPES[dt], E, H, f.data_ptr(), fe, x.data_ptr(), xe, pb, pr, re, ps, y.data_ptr(), ye,
+    check(lib.ppo2hip_glr_step(_GLR_TYPES[dt], E, H, pf, fe, px, xe, pb, pr, re, ps, y.data_ptr(), ye,
                                _raw_stream(x.get_device())), "glr_step")
     return y
+
+
+def _rows_meet(lo, hi, p, rows, step, width):
+    """Whether any of ``rows`` runs of ``width`` bytes, ``step`` bytes apart from address ``p`` on, has a byte in [lo, hi)."""
+    first = max(0, (lo - p - width) // step + 1) if step else 0         # the first that ends behind lo
+    return first < rows and lo < p + first * step + width and p + first * step < hi
 
 
 def _glr_row(t, name, shape, dtype):

@@ -206,3 +206,29 @@ def test_c_entry_refuses_bad_steps(_lib):
                dict(r=one, re=-1)):
         assert step(**kw) == _lib.EINVAL and L.ppo2hip_last_error(), kw
     assert step(E=0, s=None) == 0 and step(H=0) == 0
+
+
+def test_a_state_in_place_meets_no_input(hip):
+    """glr_step writes the state while other workgroups still read: an input in the state's memory is refused, one beside it is not."""
+    E, H = 3, 8
+    buf = z(200)
+    state = buf[40:64].view(E, H)
+    f, x = z(E, H), z(E, H)
+    rows = lambda at, step: buf.as_strided((E, H), (step, 1), at)      # noqa: E731
+    flags = lambda at, step: buf.view(torch.uint8).as_strided((E,), (step,), at)      # noqa: E731
+    for bad in (dict(x=state), dict(f=state), dict(x=rows(48, 8)), dict(f=rows(33, 0)), dict(x=rows(63, 8)), dict(f=rows(0, 20)), dict(f=rows(25, 9)),
+                dict(bias=buf[33:41]), dict(bias=buf[63:71]), dict(resets=flags(159, 1)[:E]), dict(resets=flags(100, 70)), dict(resets=flags(255, 1))):
+        args = dict(f=f, x=x, state=state)
+        args.update(bad)
+        with pytest.raises(ValueError, match="state overlaps %s" % list(bad)[0]):
+            hip.glr_step(**args)
+    # as far as the missing GPU
+    for good in (dict(x=rows(64, 8)), dict(f=rows(16, 8)), dict(x=rows(32, 32)), dict(bias=buf[32:40]), dict(bias=buf[64:72]),
+                 dict(resets=flags(157, 1)), dict(resets=flags(256, 1)), dict(resets=flags(159, 97))):
+        args = dict(f=f, x=x, state=state)
+        args.update(good)
+        with pytest.raises(TypeError, match="device tensor"):
+            hip.glr_step(**args)
+    for shape in ((0, 8), (3, 0)):
+        with pytest.raises(TypeError, match="device tensor"):
+            hip.glr_step(z(*shape), z(*shape), z(*shape))
