@@ -292,8 +292,7 @@ def glr_step(f, x, state, resets=None, bias=None, y=None):
         with torch.cuda.device(x.device):
             return glr_step(f, x, state, resets, bias, y)
     if y is None:
-        y = torch.empty_like(x)
-        ye = y.stride(0)
+        y, ye = torch.empty_like(x, memory_format=torch.contiguous_format), H          # not x's strides, whose rows may overlap
     check(lib.ppo2hip_glr_step(_GLR_TYPES[dt], E, H, pf, fe, px, xe, pb, pr, re, ps, y.data_ptr(), ye,
                                _raw_stream(x.get_device())), "glr_step")
     return y

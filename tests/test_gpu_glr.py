@@ -629,3 +629,21 @@ def test_a_chain_that_gave_up_leaves_nan(tmp_path):
     res = subprocess.run([sys.executable, str(script), root], env=env, capture_output=True, text=True, timeout=100)
     assert res.returncode == 0, res.stderr[-2000:]
     assert [l for l in res.stdout.splitlines() if l.startswith("VALUES")] == ["VALUES True"] * 2, res.stdout
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_steps_over_windows(hip, dtype):
+    """Inputs whose rows overlap: every env a window of one row, a step along; outputs have rows of their own."""
+    E, H = 5, 70
+    row = torch.randn(2, E + H, device="cuda").to(dtype)
+    f, x = (row[k].as_strided((E, H), (1, 1)) for k in range(2))
+    state = torch.randn(E, H, device="cuda")
+    want = ref.forward(f.unsqueeze(0), x.unsqueeze(0), state)[0][0]
+    tol = ref.Bounds(f.unsqueeze(0), x.unsqueeze(0), state, None, None).h
+    y = hip.glr_step(f, x, state)
+    assert y.is_contiguous()
+    close(y, want, tol, "y")
+    close(state, want, tol, "state")
+    y, last, _ = hip.glr_forward(f.expand(3, E, H), x.expand(3, E, H))
+    want = ref.forward(f.expand(3, E, H), x.expand(3, E, H))[0]
+    close(y, want, 3 * tol, "sequence")
