@@ -990,7 +990,8 @@ class AdamWPlan:
     ``grad_dtype``: type of all gradients, default each parameter's own.  ``state_bits`` 32 keeps the moments as two packed
     float32 arrays in list order (``plan.m``, ``plan.v``), 8 as codes with one float32 scale per block of 256 elements of a
     tensor (``plan.m`` int8, ``plan.v`` uint8, ``plan.m_scale``, ``plan.v_scale``): 2 bytes per parameter instead of 8.
-    ``state`` adopts existing arrays, (m, v) or (m, m_scale, v, v_scale); without it the moments start at zero.
+    ``state`` adopts existing arrays, (m, v) or (m, m_scale, v, v_scale); without it the moments start at zero.  The arrays stay
+    where they are for the plan's life: new values are copied into them.
     ``plan.norm`` is a device float32 [2]: the gradient norm (when clipping) and the factor applied to the gradients."""
 
     def __init__(self, params, state_bits=32, decay=None, state=None, grad_dtype=None):
@@ -1060,6 +1061,13 @@ class AdamWPlan:
         self._fixed = tuple(None if t is None else t.data_ptr() for t in (self._image, self.m, self.m_scale, self.v, self.v_scale, self.norm,
                                                                          self._ws))
 
+    def _check_state(self):
+        """The library goes by the addresses that the plan was made with."""
+        _, m, ms, v, vs, norm, _ = self._fixed
+        if (self.m.data_ptr() != m or self.v.data_ptr() != v or self.norm.data_ptr() != norm or
+                self.state_bits == 8 and (self.m_scale.data_ptr() != ms or self.v_scale.data_ptr() != vs)):
+            raise ValueError("moments or norm have moved since the plan was made (copy new values into them, or make a plan with state=...)")
+
     def _check_grads(self, grads):
         """One gradient or None per tensor -> the array of their addresses that the library call takes."""
         if len(grads) != len(self._ptrs):
@@ -1073,6 +1081,7 @@ class AdamWPlan:
                 raise ValueError("grads[%d] must be contiguous with %d entries" % (k, n))
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a tensor of the list has moved since the plan was made")
+        self._check_state()
         self._grads[:] = [g if g is None else g.data_ptr() or None for g in grads]
         return self._grads
 
@@ -1099,6 +1108,7 @@ def adamw_state(plan, dtype=torch.float32):
     (dtype float32); for 8-bit ones new arrays of ``dtype`` (float32 or bfloat16)."""
     if dtype not in _ADAMW_TYPES or (plan.state_bits == 32 and dtype != torch.float32):
         raise TypeError("dtype must be float32, or bfloat16 for 8-bit moments")
+    plan._check_state()
     if plan.state_bits == 32:
         return plan.m, plan.v
     if plan.device.index != torch.cuda.current_device():

@@ -450,3 +450,35 @@ def test_what_a_plan_refuses_to_share(hip):
     layer.weight.data = layer.weight.data.clone()
     with pytest.raises(ValueError, match="moved"):
         hip.adamw_step(plan, grads, 0.1, 2)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_that_were_exchanged_are_refused(hip, bits):
+    """A plan holds its arrays' addresses: a step after one of them was replaced would go on in the old one."""
+    p, grads = [torch.ones(300, device="cuda")], [torch.ones(300, device="cuda")]
+    names = ["m", "v", "norm"] + (["m_scale", "v_scale"] if bits == 8 else [])
+    for name in names:
+        for how in ("attribute", "data"):
+            plan = hip.AdamWPlan(p, state_bits=bits)
+            hip.adamw_step(plan, grads, 0.1, 1)
+            old = getattr(plan, name)
+            before = old.clone(), p[0].clone()
+            if how == "attribute":
+                setattr(plan, name, old.clone())
+            else:
+                keep = old.data         # what the plan still points at stays allocated
+                old.data = old.clone()
+            with pytest.raises(ValueError, match="moved"):
+                hip.adamw_step(plan, grads, 0.1, 2)
+            assert torch.equal(p[0], before[1])
+            if name != "norm" and bits == 8:
+                with pytest.raises(ValueError, match="moved"):
+                    hip.adamw_state(plan)
+            if how == "attribute":
+                assert torch.equal(old, before[0])
+                setattr(plan, name, old)
+                hip.adamw_step(plan, grads, 0.1, 2)
+    # new values in the same memory are what a plan takes
+    plan = hip.AdamWPlan(p, state_bits=bits)
+    plan.m.copy_(torch.ones_like(plan.m))
+    hip.adamw_step(plan, grads, 0.1, 1)
