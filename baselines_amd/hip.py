@@ -982,6 +982,11 @@ def adam_step(params, grads, m, v, lr, t, scratch, max_grad_norm=0.0, grad_scale
 _ADAMW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
+def _same_order(shape, of):
+    """Whether contiguous entries of ``shape`` stand as those of ``of`` do: the same but for dimensions of one, or flat."""
+    return (len(shape) <= 1 and shape.numel() == of.numel()) or [n for n in shape if n != 1] == [n for n in of if n != 1]
+
+
 class AdamWPlan:
     """A list of parameter tensors with their AdamW moments, laid out once for :func:`adamw_step`.
 
@@ -1021,7 +1026,7 @@ class AdamWPlan:
         self.params = params
         self.grad_dtypes = [grad_dtype or p.dtype for p in params]
         self._ptrs = [p.data_ptr() for p in params]
-        self._numels = [p.numel() for p in params]
+        self._shapes = [p.shape for p in params]
         n = len(params)
         self._tensors = (_lib.AdamwTensor * n)(*[
             _lib.AdamwTensor(p.data_ptr() if p.numel() else None, p.numel(), _ADAMW_TYPES[p.dtype], _ADAMW_TYPES[g], d, 0)
@@ -1029,7 +1034,7 @@ class AdamWPlan:
         elems = int(lib.ppo2hip_adamw_state_elements(self._tensors, n, state_bits))
         if elems < 0:
             check(elems, "adamw_state_elements")
-        self.numel = sum(self._numels)
+        self.numel = sum(p.numel() for p in params)
         blocks = elems // _lib.ADAMW_BLOCK
         with torch.cuda.device(dev):
             if state is None:
@@ -1073,12 +1078,13 @@ class AdamWPlan:
         if len(grads) != len(self._ptrs):
             raise ValueError("adamw_step needs one gradient (or None) per tensor: %d for %d" % (len(grads), len(self._ptrs)))
         gpu = self.device.index
-        for g, dt, n in zip(grads, self.grad_dtypes, self._numels):
-            if g is not None and not (isinstance(g, torch.Tensor) and g.dtype is dt and g.get_device() == gpu and g.numel() == n and g.is_contiguous()):
+        for g, dt, s in zip(grads, self.grad_dtypes, self._shapes):
+            if g is not None and not (isinstance(g, torch.Tensor) and g.dtype is dt and g.get_device() == gpu and g.shape == s and g.is_contiguous()):
                 k = next(i for i, h in enumerate(grads) if h is g)
                 if not isinstance(g, torch.Tensor) or g.dtype is not dt or g.get_device() != gpu:
                     raise TypeError("grads[%d] must be %s on %s" % (k, dt, self.device))
-                raise ValueError("grads[%d] must be contiguous with %d entries" % (k, n))
+                if not (g.is_contiguous() and _same_order(g.shape, s)):
+                    raise ValueError("grads[%d] must be contiguous with shape %s" % (k, tuple(s)))
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a tensor of the list has moved since the plan was made")
         self._check_state()
@@ -1087,8 +1093,8 @@ class AdamWPlan:
 
 
 def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, max_grad_norm=0.0, grad_scale=1.0):
-    """One AdamW step of every tensor of ``plan``: step count ``t`` (1 for the first), gradients in list order (contiguous; None
-    leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by the norm over all of them when
+    """One AdamW step of every tensor of ``plan``: step count ``t`` (1 for the first), gradients in list order (contiguous, in
+    their tensors' shapes or flat; None leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by the norm over all of them when
     ``max_grad_norm`` > 0.  Bias-corrected roots next to ``epsilon`` and decay apart from the gradient: unlike :func:`adam_step`,
     which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  Gradients must not share memory with the parameters or moments.  A
     plan's steps go one after the other, also those of HIP graphs that captured them (they share its moments and workspace); a

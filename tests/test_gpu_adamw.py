@@ -482,3 +482,20 @@ def test_moments_that_were_exchanged_are_refused(hip, bits):
     plan = hip.AdamWPlan(p, state_bits=bits)
     plan.m.copy_(torch.ones_like(plan.m))
     hip.adamw_step(plan, grads, 0.1, 1)
+
+
+def test_gradients_have_their_tensors_shapes(hip):
+    """An [H, D] gradient has as many entries as its [D, H] tensor, and none of them in its place.  Dimensions of one and flat
+    gradients change no order."""
+    p = [torch.ones(4, 6, device="cuda"), torch.ones(5, device="cuda"), torch.ones((), device="cuda")]
+    plan = hip.AdamWPlan(p)
+    z = lambda *s: torch.ones(s, device="cuda")      # noqa: E731
+    for k, bad in ((0, z(6, 4)), (0, z(2, 12)), (0, z(4, 3, 2)), (1, z(6)), (1, z(5, 2)), (2, z(2))):
+        grads = [z(4, 6), z(5), z()]
+        grads[k] = bad
+        before = [q.clone() for q in p]
+        with pytest.raises(ValueError, match=r"grads\[%d\]" % k):
+            hip.adamw_step(plan, grads, 0.1, 1)
+        assert all(torch.equal(a, b) for a, b in zip(p, before))
+    for t, grads in enumerate(([z(4, 6), z(5), z()], [z(24), z(5, 1), z(1)], [z(1, 4, 6), None, z(1, 1)]), 1):
+        hip.adamw_step(plan, grads, 0.1, t)
