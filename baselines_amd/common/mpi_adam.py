@@ -245,8 +245,11 @@ class MpiAdamW:
         if self.comm.size > 1:
             if len(grads) != len(self._views) or any(g is None for g in grads):
                 raise ValueError("every rank must bring a gradient for each of the %d tensors" % len(self._views))
+            for k, (v, g) in enumerate(zip(self._views, grads)):
+                if not self._hip.same_order(g.shape, v.shape):
+                    raise ValueError("grads[%d] must have shape %s" % (k, tuple(v.shape)))
             for v, g in zip(self._views, grads):
-                v.copy_(g)
+                v.copy_(g.reshape(v.shape))
             self.comm.allreduce_sum_(self._sum)
             grads = self._views
         scale = 1.0 / self.comm.size if self.scale_grad_by_procs else 1.0

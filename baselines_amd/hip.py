@@ -982,7 +982,7 @@ def adam_step(params, grads, m, v, lr, t, scratch, max_grad_norm=0.0, grad_scale
 _ADAMW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
-def _same_order(shape, of):
+def same_order(shape, of):
     """Whether contiguous entries of ``shape`` stand as those of ``of`` do: the same but for dimensions of one, or flat."""
     return (len(shape) <= 1 and shape.numel() == of.numel()) or [n for n in shape if n != 1] == [n for n in of if n != 1]
 
@@ -1083,7 +1083,7 @@ class AdamWPlan:
                 k = next(i for i, h in enumerate(grads) if h is g)
                 if not isinstance(g, torch.Tensor) or g.dtype is not dt or g.get_device() != gpu:
                     raise TypeError("grads[%d] must be %s on %s" % (k, dt, self.device))
-                if not (g.is_contiguous() and _same_order(g.shape, s)):
+                if not (g.is_contiguous() and same_order(g.shape, s)):
                     raise ValueError("grads[%d] must be contiguous with shape %s" % (k, tuple(s)))
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a tensor of the list has moved since the plan was made")

@@ -499,3 +499,23 @@ def test_gradients_have_their_tensors_shapes(hip):
         assert all(torch.equal(a, b) for a, b in zip(p, before))
     for t, grads in enumerate(([z(4, 6), z(5), z()], [z(24), z(5, 1), z(1)], [z(1, 4, 6), None, z(1, 1)]), 1):
         hip.adamw_step(plan, grads, 0.1, t)
+
+
+def test_mpi_adamw_gradients_of_wrong_shapes(hip):
+    """With several ranks as in a single process: nothing is broadcast into a tensor's gradient."""
+    from baselines_amd.common.mpi_adam import MpiAdamW
+    p = [torch.ones(4, 6, device="cuda"), torch.ones(5, device="cuda")]
+    a, b = [q.clone() for q in p], [q.clone() for q in p]
+    one, two = MpiAdamW(a), MpiAdamW(b, comm=_TwoRanks())
+    z = lambda *s: torch.rand(s, device="cuda")      # noqa: E731
+    for k, bad in ((0, z(6)), (0, z(1)), (0, z(6, 4)), (0, z(4, 1)), (1, z(1)), (1, z())):
+        grads = [z(4, 6), z(5)]
+        grads[k] = bad
+        for opt in (one, two):
+            with pytest.raises(ValueError, match=r"grads\[%d\]" % k):
+                opt.update(grads, 0.1)
+        assert one.t == two.t == 0
+    for grads in ([z(4, 6), z(5)], [z(24), z(5, 1)]):
+        one.update(grads, 0.1)
+        two.update(grads, 0.1)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
