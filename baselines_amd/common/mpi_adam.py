@@ -21,6 +21,8 @@ Two sharding modes (envs shard by index in both, so GAE needs no communication):
              and the ranks all-reduce {sum a, sum a^2, n} and un-normalised gradient sums, so
              N ranks reproduce the single-process update up to summation order.
 """
+import operator
+
 import numpy as np
 import torch
 import torch.distributed as dist
@@ -215,13 +217,14 @@ class MpiAdamW:
     (mpi_adam.py:22-23), sums the gradients over the ranks, scales by 1/size (``scale_grad_by_procs``, :27-28), clips by the
     global norm when ``max_grad_norm`` > 0 and steps every tensor in one kernel launch; ``sync`` broadcasts rank 0's
     parameters (:37-40).  ``params``, ``decay``, ``state_bits`` (32, or 8 for moments in codes) and ``state`` are those of
-    ``hip.AdamWPlan``, held in ``self.plan``.
+    ``hip.AdamWPlan``, held in ``self.plan``; ``t`` counts the steps that an adopted ``state`` has taken (its bias corrections go
+    by it).
 
     A gradient may be None (its tensor is left out of the step) in a single process only: ranks add one packed float32
     buffer, so each of them has to bring every gradient."""
 
     def __init__(self, params, *, beta1=0.9, beta2=0.999, epsilon=1e-08, weight_decay=0.01, decay=None, state_bits=32,
-                 max_grad_norm=0.0, scale_grad_by_procs=True, comm=None, state=None, grad_dtype=None):
+                 max_grad_norm=0.0, scale_grad_by_procs=True, comm=None, state=None, grad_dtype=None, t=0):
         from .. import hip
         self._hip = hip
         self.comm = comm or DataParallel("mpi")
@@ -229,10 +232,12 @@ class MpiAdamW:
         self.max_grad_norm = max_grad_norm
         self.scale_grad_by_procs = scale_grad_by_procs
         self.params = list(params)
+        self.t = operator.index(t)
+        if self.t < 0:
+            raise ValueError("t must not be negative")
         if self.comm.size > 1:
             grad_dtype = torch.float32           # the type of the buffer that the ranks add up
         self.plan = hip.AdamWPlan(self.params, state_bits=state_bits, decay=decay, state=state, grad_dtype=grad_dtype)
-        self.t = 0
         self._sum = self._views = None
         if self.comm.size > 1:
             self._sum = torch.empty(self.plan.numel, dtype=torch.float32, device=self.plan.device)

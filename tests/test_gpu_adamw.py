@@ -519,3 +519,25 @@ def test_mpi_adamw_gradients_of_wrong_shapes(hip):
         one.update(grads, 0.1)
         two.update(grads, 0.1)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_mpi_adamw_goes_on_from_adopted_state(hip):
+    """Three steps, and two more by a second object that takes the first one's moments and its count: five steps in a row."""
+    from baselines_amd.common.mpi_adam import MpiAdamW
+    g = torch.Generator(device="cuda").manual_seed(3)
+    start = tensors([64, 300], F32, g)
+    grads = [tensors([64, 300], F32, g) for _ in range(5)]
+    one, two = [p.clone() for p in start], [p.clone() for p in start]
+    a, b = MpiAdamW(one), MpiAdamW(two)
+    for k in range(5):
+        a.update(grads[k], 1e-2)
+    for k in range(3):
+        b.update(grads[k], 1e-2)
+    c = MpiAdamW(two, state=(b.plan.m, b.plan.v), t=b.t)
+    for k in (3, 4):
+        c.update(grads[k], 1e-2)
+    assert c.t == 5
+    assert all(torch.equal(p, q) for p, q in zip(one, two)) and torch.equal(a.plan.m, c.plan.m) and torch.equal(a.plan.v, c.plan.v)
+    for t in (-1, 1.5, None):
+        with pytest.raises((ValueError, TypeError)):
+            MpiAdamW(two, t=t)
