@@ -647,3 +647,65 @@ def test_steps_over_windows(hip, dtype):
     y, last, _ = hip.glr_forward(f.expand(3, E, H), x.expand(3, E, H))
     want = ref.forward(f.expand(3, E, H), x.expand(3, E, H))[0]
     close(y, want, 3 * tol, "sequence")
+
+
+def walks_back(hip, dtype, E, H):
+    """Whether the gradients of so many columns go back with one wave per tile: a long sequence then needs no workspace."""
+    from baselines_amd import _lib
+    return _lib.lib.ppo2hip_glr_backward_workspace_bytes(hip._GLR_TYPES[dtype], 300, E, H, 0) == 0
+
+
+@pytest.mark.parametrize("T,E,H,kind", [(1, 2500, 33, "apart"), (16, 1300, 64, "apart"), (17, 640, 129, "joint"), (40, 330, 256, "batch first"), (300, 330, 250, "apart"),
+                                        (270, 2, 41000, "odd"), (33, 81920, 1, "apart")])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_many_columns_in_16_bits(hip, T, E, H, kind, dtype):
+    """Gradients that a wave walks back by itself over all steps of its columns, from one span to many, the last one cut short."""
+    assert walks_back(hip, dtype, E, H)
+    k = T + E + H
+    a, normal = make(T, E, H, dtype, kind=kind, resets=k % 2 == 0, bias=k % 3 != 0, h0=k % 5 != 0, seed=k)
+    check(hip, a, normal, dtype, kind, dh_last=k % 7 != 0)
+    if a["bias"] is None or a["resets"] is None:
+        a, normal = make(T, E, H, dtype, kind=kind, resets=True, bias=True, seed=k)
+        check(hip, a, normal, dtype, kind)
+
+
+@pytest.mark.parametrize("T", [5, 40, 300])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_what_a_reset_hides_from_many_columns(hip, T, dtype):
+    E, H, r = 3, 27500, T // 2
+    assert walks_back(hip, dtype, E, H)
+    a, normal = make(T, E, H, dtype, bias=True)
+    a["resets"] = torch.zeros(T, E, dtype=torch.uint8, device="cuda")
+    a["resets"][r] = 1
+    dy = normal(T, E, H).to(dtype)
+    clean = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    gclean = hip.glr_backward(a["f"], a["x"], dy, clean[2], resets=a["resets"], bias=a["bias"])
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        h0, x, dyb = a["h0"].clone(), a["x"].clone(), dy.clone()
+        h0[0, 3] = bad
+        x[r - 1, 1, 5] = bad
+        dyb[r, 2, H - 1] = bad
+        y, last, saved = hip.glr_forward(a["f"], x, h0, resets=a["resets"], bias=a["bias"], want_saved=True)
+        assert torch.equal(y[r:], clean[0][r:]) and torch.equal(last, clean[1])
+        df, dx, dh0, _ = hip.glr_backward(a["f"], x, dyb, saved, resets=a["resets"], bias=a["bias"])
+        assert torch.equal(dx[:r], gclean[1][:r]) and torch.equal(dh0, gclean[2])
+        assert torch.equal(df[r + 1:], gclean[0][r + 1:])
+        rest = torch.ones_like(df, dtype=torch.bool)
+        rest[:r, 0, 3] = False
+        rest[:r, 1, 5] = False
+        rest[r, 2, H - 1] = False
+        assert torch.equal(df[rest], gclean[0][rest])
+
+
+def test_many_columns_of_envs_far_apart(hip):
+    """Envs 2^29 elements apart: each has tiles of its own, the last one of 40 columns."""
+    T, E, H = 20, 2, 41000
+    se = 1 << 29
+    assert walks_back(hip, BF16, E, H)
+    buf = torch.empty((E - 1) * se + T * H * 2 + 8, dtype=BF16, device="cuda")
+    views = [buf.as_strided((T, E, H), (2 * H, se, 1), k * H) for k in range(2)]
+    a, normal = make(T, E, H, BF16, resets=True, bias=True)
+    for v, t in zip(views, (a["f"], a["x"])):
+        v.copy_(t)
+    a["f"], a["x"] = views
+    check(hip, a, normal, BF16)
