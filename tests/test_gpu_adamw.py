@@ -541,3 +541,60 @@ def test_mpi_adamw_goes_on_from_adopted_state(hip):
     for t in (-1, 1.5, None):
         with pytest.raises((ValueError, TypeError)):
             MpiAdamW(two, t=t)
+
+
+# chunks of 2048 elements: 601 (a norm whose workgroups take more than one, its sums added up by every workgroup of the step), 2101
+# (more sums than those add up: a launch of its own finds norm and factor), and both over lists of more than one launch's tensors
+WIDE = [[600 * 2048 + 5], [2100 * 2048 + 7], [3, 2049 * 2048, 1], [5 * 2048 - 3] * 500, [700] * 1000 + [1500 * 2048 + 1]]
+
+
+@pytest.mark.parametrize("sizes", WIDE, ids=lambda s: "%dx%d" % (len(s), max(s)))
+@pytest.mark.parametrize("pt", [F32, BF16])
+@pytest.mark.parametrize("clip", [0.0, 0.5])
+def test_wide_lists_32_bits(hip, sizes, pt, clip):
+    test_32_bits(hip, sizes, pt, F32, clip)
+
+
+@pytest.mark.parametrize("sizes", WIDE, ids=lambda s: "%dx%d" % (len(s), max(s)))
+@pytest.mark.parametrize("clip", [0.0, 0.5, 1e9])
+def test_wide_lists_8_bits(hip, sizes, clip):
+    test_8_bits(hip, sizes, F32, F32, clip)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    plan = hip.AdamWPlan(tensors(sizes, F32, g, 0.1), state_bits=8)
+    grads = tensors(sizes, F32, g, 0.3)
+    for t, none in enumerate((None, len(sizes) // 2), 1):
+        if none is not None:
+            grads[none] = None
+        before = [p.clone() for p in plan.params], plan.m.clone()
+        hip.adamw_step(plan, grads, 0.1, t, max_grad_norm=clip, grad_scale=2.0)
+        norm = sum(float(x.double().square().sum()) for x in grads if x is not None) ** 0.5 * 2.0
+        factor = min(1.0, clip / norm) if clip and norm else 1.0
+        if clip:
+            assert abs(float(plan.norm[0]) - norm) <= 4 * U * norm
+        assert abs(float(plan.norm[1]) - 2.0 * factor) <= 16 * U * factor
+        for k in range(len(sizes)):
+            if k == none:
+                assert torch.equal(plan.params[k], before[0][k])
+        if none is not None:
+            assert torch.equal(unpad(plan.m, sizes)[none], unpad(before[1], sizes)[none])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_wide_lists_captured_and_replayed(hip, bits):
+    """The three launches of a wide clipped list in a graph, replayed with new gradients, against eager steps."""
+    sizes = [2100 * 2048 + 7, 300]
+    g = torch.Generator(device="cuda").manual_seed(9)
+    start, grads = tensors(sizes, F32, g), tensors(sizes, F32, g)
+    pg, pe = [p.clone() for p in start], [p.clone() for p in start]
+    plan_g, plan_e = hip.AdamWPlan(pg, state_bits=bits), hip.AdamWPlan(pe, state_bits=bits)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hip.adamw_step(plan_g, grads, 1e-2, 7, max_grad_norm=0.5)
+    for _ in range(4):
+        for x in grads:
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        hip.adamw_step(plan_e, grads, 1e-2, 7, max_grad_norm=0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(pg + [plan_g.m, plan_g.v, plan_g.norm], pe + [plan_e.m, plan_e.v, plan_e.norm]))
