@@ -95,7 +95,7 @@ struct Run<false> {
     float w[2];
     static __device__ inline float live(float A) { return fmaxf(A, 0x1p-149f); }
     static __device__ inline Run none() { return {{1.f, 0.f}}; }
-    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? 0.f : live(A > 0.5f ? 1.f - D : A), 0.f}}; }
+    static __device__ inline Run of(float A, float D, bool reset) { return {{reset ? 0.f : live(A > 0.75f ? 1.f - D : A), 0.f}}; }
     __device__ inline void add(float B) { w[1] = B; }
     __device__ inline float through(float h) const { return w[0] == 0.f ? w[1] : fmaf(w[0], h, w[1]); }
     __device__ inline Run join(const Run &r) const { return {{r.w[0] == 0.f || w[0] == 0.f ? 0.f : live(w[0] * r.w[0]), r.through(w[1])}}; }
@@ -329,7 +329,7 @@ __device__ inline void span_walk(const Span<V> &g, const Span<V> &u, unsigned rm
 }
 
 // What a span lets through.  D = 1 - A grows by 1 - a of what is left of it, so that it keeps its figures while it is small.  For 16
-// bits D counts only where A ends above 1/2, which no gate below 1/2 leaves it: there 1 - a is the gate as it is held, negated.
+// bits D counts only where A ends above 3/4, which no gate of 1/2 and less leaves it: there 1 - a is the gate as it is held, negated.
 template <bool EXACT, int V>
 __device__ inline void span_passes(const Span<V> &g, unsigned rm, Run<EXACT> (&r)[V]) {
     typedef Gate<EXACT> G;

@@ -709,3 +709,20 @@ def test_many_columns_of_envs_far_apart(hip):
         v.copy_(t)
     a["f"], a["x"] = views
     check(hip, a, normal, BF16)
+
+
+@pytest.mark.parametrize("T", [20, 300])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_gates_around_one_half(hip, T, dtype):
+    """f + bias at and next to zero, from either side, where a gate is held by its other side: a run of such gates between two that
+    keep everything, and runs with only one of them."""
+    near = [0.0, -0.0, 2.0 ** -24, -2.0 ** -24, 3e-7, -3e-7, 1e-5, -1e-5, 2.0 ** -120, -2.0 ** -120, 0.7, -0.7, 1.1, 1.09]
+    bias = torch.tensor(near, device="cuda")
+    f = torch.full((T, 3, len(near)), 40.0, device="cuda").to(dtype)
+    f[5, 0] = 0.0                                   # one gate of the span
+    f[3:17, 1] = 0.0
+    f[:, 2] = 0.0
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x, dy = (torch.randn(f.shape, generator=g, device="cuda").to(dtype) for _ in range(2))
+    h0 = torch.randn(3, len(near), generator=g, device="cuda")
+    check(hip, dict(f=f, x=x, h0=h0, resets=None, bias=bias), lambda *s: torch.randn(s, generator=g, device="cuda"), dtype)
