@@ -982,9 +982,13 @@ def adam_step(params, grads, m, v, lr, t, scratch, max_grad_norm=0.0, grad_scale
 _ADAMW_TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16}
 
 
+def _flat(shape):
+    return sum(n != 1 for n in shape) <= 1
+
+
 def same_order(shape, of):
-    """Whether contiguous entries of ``shape`` stand as those of ``of`` do: the same but for dimensions of one, or flat."""
-    return (len(shape) <= 1 and shape.numel() == of.numel()) or [n for n in shape if n != 1] == [n for n in of if n != 1]
+    """Whether contiguous entries of ``shape`` stand as those of ``of`` do: the same but for dimensions of one, or either flat."""
+    return shape.numel() == of.numel() and (_flat(shape) or _flat(of) or [n for n in shape if n != 1] == [n for n in of if n != 1])
 
 
 class AdamWPlan:
@@ -1022,11 +1026,12 @@ class AdamWPlan:
         for k, p in enumerate(params):
             if not p.is_cuda or p.device != dev:
                 raise TypeError("params[%d] must be a tensor of the first one's GPU" % k)
-        self.device, self.state_bits = dev, state_bits
+        self.device, self._gpu, self.state_bits = dev, dev.index, state_bits
         self.params = params
         self.grad_dtypes = [grad_dtype or p.dtype for p in params]
         self._ptrs = [p.data_ptr() for p in params]
-        self._shapes = [p.shape for p in params]
+        self._numels = [p.numel() for p in params]
+        self._shapes = [None if _flat(p.shape) else p.shape for p in params]
         n = len(params)
         self._tensors = (_lib.AdamwTensor * n)(*[
             _lib.AdamwTensor(p.data_ptr() if p.numel() else None, p.numel(), _ADAMW_TYPES[p.dtype], _ADAMW_TYPES[g], d, 0)
@@ -1034,7 +1039,7 @@ class AdamWPlan:
         elems = int(lib.ppo2hip_adamw_state_elements(self._tensors, n, state_bits))
         if elems < 0:
             check(elems, "adamw_state_elements")
-        self.numel = sum(p.numel() for p in params)
+        self.numel = sum(self._numels)
         blocks = elems // _lib.ADAMW_BLOCK
         with torch.cuda.device(dev):
             if state is None:
@@ -1073,18 +1078,26 @@ class AdamWPlan:
                 self.state_bits == 8 and (self.m_scale.data_ptr() != ms or self.v_scale.data_ptr() != vs)):
             raise ValueError("moments or norm have moved since the plan was made (copy new values into them, or make a plan with state=...)")
 
+    def _check_grad(self, k, g):
+        if not isinstance(g, torch.Tensor) or g.dtype is not self.grad_dtypes[k] or g.get_device() != self._gpu:
+            raise TypeError("grads[%d] must be %s on %s" % (k, self.grad_dtypes[k], self.device))
+        if not (g.is_contiguous() and same_order(g.shape, self.params[k].shape)):
+            raise ValueError("grads[%d] must be contiguous with shape %s" % (k, tuple(self.params[k].shape)))
+
     def _check_grads(self, grads):
         """One gradient or None per tensor -> the array of their addresses that the library call takes."""
         if len(grads) != len(self._ptrs):
             raise ValueError("adamw_step needs one gradient (or None) per tensor: %d for %d" % (len(grads), len(self._ptrs)))
-        gpu = self.device.index
-        for g, dt, s in zip(grads, self.grad_dtypes, self._shapes):
-            if g is not None and not (isinstance(g, torch.Tensor) and g.dtype is dt and g.get_device() == gpu and g.shape == s and g.is_contiguous()):
-                k = next(i for i, h in enumerate(grads) if h is g)
-                if not isinstance(g, torch.Tensor) or g.dtype is not dt or g.get_device() != gpu:
-                    raise TypeError("grads[%d] must be %s on %s" % (k, dt, self.device))
-                if not (g.is_contiguous() and same_order(g.shape, s)):
-                    raise ValueError("grads[%d] must be contiguous with shape %s" % (k, tuple(s)))
+        gpu = self._gpu
+        try:
+            for g, dt, n, s in zip(grads, self.grad_dtypes, self._numels, self._shapes):
+                if g is not None and not (g.dtype is dt and g.get_device() == gpu and g.numel() == n and g.is_contiguous() and (s is None or g.shape == s)):
+                    for k, h in enumerate(grads):
+                        if h is not None:
+                            self._check_grad(k, h)
+                    break
+        except AttributeError:
+            raise TypeError("a gradient is a tensor or None") from None
         if [p.data_ptr() for p in self.params] != self._ptrs:
             raise ValueError("a tensor of the list has moved since the plan was made")
         self._check_state()
@@ -1099,14 +1112,15 @@ def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_
     which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  Gradients must not share memory with the parameters or moments.  A
     plan's steps go one after the other, also those of HIP graphs that captured them (they share its moments and workspace); a
     captured call keeps ``lr``, ``t`` and the gradients' addresses."""
-    if plan.device.index != torch.cuda.current_device():
+    gpu = plan._gpu
+    if gpu != torch._C._cuda_getDevice():
         with torch.cuda.device(plan.device):
             return adamw_step(plan, grads, lr, t, beta1, beta2, epsilon, weight_decay, max_grad_norm, grad_scale)
     ptrs = plan._check_grads(grads)
     image, m, ms, v, vs, norm, ws = plan._fixed
     check(lib.ppo2hip_adamw_step(plan._tensors, len(ptrs), plan.state_bits, image, ptrs, m, ms, v, vs, lr, t, beta1, beta2, epsilon,
                                  weight_decay, grad_scale, max_grad_norm or 0.0, norm, ws, plan._ws_bytes,
-                                 _raw_stream(plan.device.index)), "adamw_step")
+                                 _raw_stream(gpu)), "adamw_step")
 
 
 def adamw_state(plan, dtype=torch.float32):

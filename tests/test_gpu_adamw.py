@@ -499,6 +499,11 @@ def test_gradients_have_their_tensors_shapes(hip):
         assert all(torch.equal(a, b) for a, b in zip(p, before))
     for t, grads in enumerate(([z(4, 6), z(5), z()], [z(24), z(5, 1), z(1)], [z(1, 4, 6), None, z(1, 1)]), 1):
         hip.adamw_step(plan, grads, 0.1, t)
+    one = z(4, 6)                                   # the same tensor twice: right for the first, wrong for the second
+    plan = hip.AdamWPlan([z(4, 6), z(6, 4)])
+    with pytest.raises(ValueError, match=r"grads\[1\]"):
+        hip.adamw_step(plan, [one, one], 0.1, 1)
+    hip.adamw_step(plan, [one, one.view(6, 4)], 0.1, 1)
 
 
 def test_mpi_adamw_gradients_of_wrong_shapes(hip):
