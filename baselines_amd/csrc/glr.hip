@@ -120,7 +120,12 @@ struct Lane {
     static __device__ inline void store(void *p, const float (&v)[V]) {
         Out r;
 #pragma unroll
-        for (int k = 0; k < V; k++) r[k] = (T)v[k];       // to nearest: the type that the layer hands on; states stay float32
+        for (int k = 0; k < V; k++) {
+            float w = v[k];
+            // float32 first: a product fused with its rounding to float16 rounds once, and not the same in two places
+            if (std::is_same<T, _Float16>::value) asm("" : "+v"(w));
+            r[k] = (T)w;                                  // to nearest: the type that the layer hands on; states stay float32
+        }
         *(AnyOut *)p = r;
     }
 };
@@ -694,10 +699,7 @@ __device__ inline void forward_span(const ForwardArgs<T> &a, const Place &at, un
 #pragma unroll
             for (int i = 0; i < kSpan; i++) {
 #pragma unroll
-                for (int k = 0; k < V; k++) {
-                    v[k] = fmaf(g[i][k], h[k], u[i][k]);
-                    asm("" : "+v"(v[k]));                   // float32 first: fused with its rounding to 16 bits it is not the slow way's
-                }
+                for (int k = 0; k < V; k++) v[k] = fmaf(g[i][k], h[k], u[i][k]);
                 put(i, v);
             }
         } else {

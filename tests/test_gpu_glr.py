@@ -726,3 +726,24 @@ def test_gates_around_one_half(hip, T, dtype):
     x, dy = (torch.randn(f.shape, generator=g, device="cuda").to(dtype) for _ in range(2))
     h0 = torch.randn(3, len(near), generator=g, device="cuda")
     check(hip, dict(f=f, x=x, h0=h0, resets=None, bias=bias), lambda *s: torch.randn(s, generator=g, device="cuda"), dtype)
+
+
+@pytest.mark.parametrize("T,E,H", [(9000, 2, 70), (100, 30, 70)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_column_that_is_no_number_changes_no_other(hip, T, E, H, dtype):
+    """A wave that walks a span the slow way for one of its columns rounds the others' outputs as the quick way does."""
+    a, normal = make(T, E, H, dtype, bias=True)
+    dy = normal(T, E, H).to(dtype)
+
+    def both(x, dy):
+        y, last, saved = hip.glr_forward(a["f"], x, a["h0"], bias=a["bias"], want_saved=True)
+        return (y, last) + hip.glr_backward(a["f"], x, dy, saved, bias=a["bias"])
+    clean = both(a["x"], dy)
+    x, dyb = a["x"].clone(), dy.clone()
+    x[1, 1, 5], dyb[T - 2, 0, 9] = float("nan"), float("inf")
+    got = both(x, dyb)
+    ok = torch.ones(E, H, dtype=torch.bool, device="cuda")
+    ok[1, 5] = ok[0, 9] = False
+    for g, c in zip(got[:5], clean[:5]):
+        assert torch.equal(g[ok] if g.dim() == 2 else g[:, ok], c[ok] if c.dim() == 2 else c[:, ok])
+    assert torch.equal(got[5][ok.all(0)], clean[5][ok.all(0)])
