@@ -420,7 +420,10 @@ __device__ inline void span_scan(const Args &a, const Place &at, const Raw<T, V>
                 }
             }
 #pragma unroll
-            for (int k = 0; k < V; k++) u[i][k] = h[k];
+            for (int k = 0; k < V; k++) {
+                u[i][k] = h[k];
+                if (anew(rm) << (31 - i)) g[i][k] = 0.f;    // a reset at step i or before also hides a gate that is no number
+            }
         }
     }
 #pragma unroll

@@ -747,3 +747,32 @@ def test_a_column_that_is_no_number_changes_no_other(hip, T, E, H, dtype):
     for g, c in zip(got[:5], clean[:5]):
         assert torch.equal(g[ok] if g.dim() == 2 else g[:, ok], c[ok] if c.dim() == 2 else c[:, ok])
     assert torch.equal(got[5][ok.all(0)], clean[5][ok.all(0)])
+
+
+@pytest.mark.parametrize("T,E,H", [(5, 2, 70), (40, 3, 33), (700, 2, 70), (9000, 2, 70), (40, 3, 27500)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("gap", [1, 3])
+def test_a_reset_hides_gates_that_are_no_numbers(hip, T, E, H, dtype, gap):
+    """A gate that is no number some steps in front of a reset: its column from there up to the reset, forward, and from there back to the
+    reset before, backward; everything else bit for bit."""
+    r = T // 2
+    a, normal = make(T, E, H, dtype, bias=True)
+    a["resets"] = torch.zeros(T, E, dtype=torch.uint8, device="cuda")
+    a["resets"][r] = 1
+    a["resets"][0] = 1
+    dy = normal(T, E, H).to(dtype)
+    clean = hip.glr_forward(a["f"], a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    gclean = hip.glr_backward(a["f"], a["x"], dy, clean[2], resets=a["resets"], bias=a["bias"])
+    f, at = a["f"].clone(), max(r - gap, 0)
+    f[at, 1, 5] = float("nan")
+    y, last, saved = hip.glr_forward(f, a["x"], a["h0"], resets=a["resets"], bias=a["bias"], want_saved=True)
+    df, dx, dh0, dbias = hip.glr_backward(f, a["x"], dy, saved, resets=a["resets"], bias=a["bias"])
+    assert bool(torch.isnan(y[at:r, 1, 5]).all()) and bool(torch.isnan(df[:r, 1, 5]).any())
+    rest = torch.ones_like(y, dtype=torch.bool)
+    rest[at:r, 1, 5] = False
+    assert torch.equal(y[rest], clean[0][rest]) and torch.equal(last, clean[1])
+    rest[:r, 1, 5] = False
+    assert torch.equal(df[rest], gclean[0][rest]) and torch.equal(dx[rest], gclean[1][rest]) and torch.equal(dh0, gclean[2])
+    ok = torch.ones(H, dtype=torch.bool, device="cuda")
+    ok[5] = False
+    assert torch.equal(dbias[ok], gclean[3][ok]) and bool(torch.isnan(dbias[5]))
