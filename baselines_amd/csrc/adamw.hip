@@ -16,8 +16,12 @@ constexpr int kChunk = 2048;                     // elements a workgroup takes a
 constexpr int kThreads = 256;
 constexpr int kMaxGrads = 448;                   // gradient pointers of one launch: they ride in its 4 KB of arguments
 constexpr int kNormGroups = 4096;                // most workgroups of the norm launch, each with a partial sum
-constexpr int kOwnSums = 512;                    // most partial sums that every workgroup of the step adds up by itself
-constexpr int kOwnChunks = 2048;                 // chunks from which it does not
+// Up to kOwnChunks chunks every workgroup of the step adds up the norm's partial sums, kOwnSums at most, by itself; beyond, one more
+// launch does.  By itself / by the launch, us per replay, 32-bit and 8-bit moments: 64 chunks 7.6 / 8.9 and 10.0 / 11.3, 512: 10.0 /
+// 11.0 and 11.5 / 12.6, 2048: 24.7 / 25.9 and 25.7 / 25.7, 4096: 46.5 / 47.0 and 43.1 / 41.1, 8192: 92 / 87 and 74 / 65.  256, 512, 1024 sums:
+// 1235 chunks 17.8, 17.0, 16.5 and 17.4, 16.9, 17.1, 2048 chunks 28.1, 24.7, 24.4 and 28.2, 25.7, 25.2.
+constexpr int kOwnSums = 512;
+constexpr int kOwnChunks = 2048;
 constexpr int kSmallThreads = 1024, kSmallChunks = 32;   // chunks up to which every workgroup of the step sums all squares itself
 
 struct TensorRow {                               // one tensor in the device image of a plan
@@ -216,10 +220,10 @@ __device__ inline float over_root(float m, float v, float eps) {
 
 // THREADS kThreads: a workgroup per chunk.  kSmallThreads, for lists of at most kSmallChunks chunks that are clipped: the same,
 // after its waves have summed the squares of the whole list, so that the norm needs no launch of its own.  In one launch / in two, us
-// per replay and per eager call, 32-bit moments: 8 chunks 5.1 and 9.5 / -, 24 chunks 6.5 and 9.0 / 7.1 and 12.2, 32 chunks 7.9 and
-// 9.0 / 7.2 and 12.5, 64 chunks 11.5 and 11.7 / 7.2 and 12.6; 8-bit, 32 chunks: 8.7 and 9.3 / 9.3 and 12.3.
-// Bound by memory: 126 M parameters in 100 tensors, float32 moments 3.5 GB in 638 us (5.5 TB/s), 8 bits 2.0 GB in 350 (5.8); 43 M
-// bfloat16 ones 1.0 GB in 181 (5.3).
+// per replay, 32-bit moments: 24 chunks 6.5 / 7.1, 32 chunks 7.9 / 7.2, 64 chunks 11.5 / 7.2; 8-bit, 32 chunks: 8.7 / 9.3.  An eager
+// call, which waits for the host, takes 3 us less in one.
+// Bound by memory: 126 M parameters in 100 tensors, float32 moments 3.5 GB in 638 us (5.5 TB/s), 8 bits 2.0 GB in 355 (5.7); 43 M
+// bfloat16 ones 1.0 GB in 182 (5.3).
 template <int BITS, int THREADS>
 __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a) {
     constexpr int kParts = (kChunk + 4 * THREADS - 1) / (4 * THREADS);
@@ -306,7 +310,7 @@ __global__ __launch_bounds__(THREADS) void adamw_kernel(AdamwArgs a) {
     }
 }
 
-// moments as the values they stand for, packed in list order (no padding between tensors): 126 M, 760 MB in 147 us (5.2 TB/s)
+// moments as the values they stand for, packed in list order (no padding between tensors): 126 M, 760 MB in 151 us (5.0 TB/s)
 template <class T>
 __global__ __launch_bounds__(kThreads) void adamw_state_kernel(const TensorRow *tensors, const ChunkRow *chunks, const int64_t *packed, int nchunks,
                                                                const unsigned *mc_, const unsigned *vc_, const float *m_scale, const float *v_scale,

@@ -10,7 +10,8 @@
 #include "kernels.hpp"
 
 // Products and sums round one by one unless fmaf says otherwise: the same step written in two places gives the same bits, so
-// that a state recomputed in the backward pass is the forward's, and a span walked the slow way changes no other column.
+// that a span walked the slow way changes no other column, and the states that the backward pass recomputes are those that forward
+// walked (a chain in 16 bits puts its outputs together from products instead, a few roundings of float32 from them).
 #pragma clang fp contract(off)
 
 namespace ppo2hip {
@@ -182,7 +183,7 @@ __device__ inline Place place_of(unsigned tile, unsigned C, unsigned H, unsigned
 }
 // Tile of a workgroup.  Workgroups go to the 8 XCDs in turn, and rows whose length is no multiple of a cache line leave
 // neighbouring tiles with a line in common: eight tiles in a row are given to one XCD, whose L2 then fetches and merges it once.
-// [200, 300, 777] bfloat16: 84 / 167 us forward / backward without, 71 / 141 with.
+// [200, 300, 777] bfloat16: 103 / 204 us forward / backward without, 90 / 181 with.
 __device__ inline unsigned seat_of(unsigned b) { return (b | 63u) < gridDim.x ? (b & ~63u) | (b & 7) << 3 | (b >> 3 & 7) : b; }
 template <class T>
 __device__ inline unsigned lane_offset(const Seq<T> &s, const Place &at) {
@@ -487,9 +488,9 @@ struct RunSpace {
 // Four tiles in a row share a counter, behind which their batches are given out in order, all four tiles' first ones before the second
 // ones: what a batch waits for, earlier batches of its own tile, has been drawn by workgroups that are running and that wait for still
 // earlier ones only, whatever else runs on the card and wherever workgroups start.  One counter for all tiles is drawn from once in
-// 10 ns: [2048, 16, 512] float32 50 us, a counter per four tiles 43, per tile 44 and [16384, 4, 1024] bfloat16 95, 97, 100 (tiles
-// that drift apart in time share no cache lines).  Lists of seats per XCD were 113 us for [65536, 1, 1000] bfloat16 where this takes
-// 125, but a workgroup then waits for seats that no running one has drawn, which two such launches at once can turn into a deadlock.
+// 10 ns: [2048, 16, 512] float32 48 us forward, a counter per four tiles 41, per tile 41 and [16384, 4, 1024] bfloat16 102, 104, 110
+// (tiles that drift apart in time share no cache lines).  Lists of seats per XCD took 14 us off [65536, 1, 1000] bfloat16, but a
+// workgroup then waits for seats that no running one has drawn, which two such launches at once can turn into a deadlock.
 constexpr int kChainWaves = 8, kBatch = kChainWaves * kSpan;
 constexpr unsigned kEmpty = 0xffffffffu;
 constexpr int kTurnWords = 64, kTurns = 64, kTurnTiles = 4, kTurnBytes = kTurns * kTurnWords * sizeof(unsigned);
@@ -726,7 +727,7 @@ __device__ inline void forward_span(const ForwardArgs<T> &a, const Place &at, un
 }
 
 // Short sequences in one launch: a workgroup holds the whole of its columns, one span per wave, and the waves exchange their
-// spans' runs through LDS.  Bound by memory: [128, 512, 256] bfloat16, 101 MB in 23.5 us, float32 and training 206 MB in 48 us (4.3 TB/s).
+// spans' runs through LDS.  Bound by memory: [128, 512, 256] bfloat16, 101 MB in 25 us, float32 and training 206 MB in 48 us (4.3 TB/s).
 template <class T, int V>
 __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArgs<T> a) {
     __shared__ RunSpace<sizeof(T) == 4, V> runs[kHeld];
@@ -755,10 +756,10 @@ __global__ __launch_bounds__(64 * kHeld) void glr_forward_held_kernel(ForwardArg
     forward_span<T, V, false>(a, at, lane_offset(a.y, at), t0, n, rm, g, u, r, h);
 }
 
-// Bound by what of the loads and the hand-over the 16 waves of a CU do not hide from each other: of 12 us that a workgroup lives, 3.2
-// are loads, 1.2 the draw, 0.5 the gates, 5 waits.  bfloat16 [65536, 1, 1000], 393 MB: 122 us (3.2 TB/s; a copy in the same tiles 102: rows
-// of 2000 bytes, whose lines neighbouring tiles fetch twice), [65536, 1, 1024] 106, [16384, 4, 1024] 96.  Two channels per lane:
-// with one 11 and 5 us more.  Waves of a workgroup: 4, 16: 151, 112 us where 8 took 107.
+// Bound by what of the loads and the hand-over the 16 waves of a CU do not hide from each other, and 31 operations per element (55 us
+// of all SIMDs for 66 M elements).  bfloat16 [65536, 1, 1000], 393 MB: 125 us (3.1 TB/s; a copy in the same tiles 102: rows of 2000
+// bytes, whose lines neighbouring tiles fetch twice), [65536, 1, 1024] 107, [16384, 4, 1024] 100.  Two channels per lane: with one 139,
+// 115, 107.  Waves of a workgroup: with 4 and 16 in place of 8 154 and 152, 131 and 139, 111 and 129.
 template <class T, int V>
 __global__ __launch_bounds__(64 * kChainWaves, V == 2 ? 4 : 5) void glr_forward_chain_kernel(ForwardArgs<T> a, Chain ch) {
     __shared__ ChainSpace<sizeof(T) == 4, V> mem;
@@ -944,7 +945,7 @@ __device__ inline void backward_walk(const BackwardArgs<T> &a, const Place &at, 
     }
 }
 
-// Many 16-bit columns: a wave per tile.  [2048, 512, 256] bfloat16, 2.7 GB in 630 us (4.3 TB/s).
+// Many 16-bit columns: a wave per tile.  [2048, 512, 256] bfloat16, 2.7 GB in 665 us (4.1 TB/s).
 template <class T>
 __global__ __launch_bounds__(64, 2) void glr_backward_kernel(BackwardArgs<T> a) {
     const Place at = place_of<1>(seat_of(blockIdx.x), a.C, a.H, a.env_tiles);
@@ -982,8 +983,8 @@ __global__ __launch_bounds__(64 * kHeld) void glr_backward_held_kernel(BackwardA
     if (a.dbias_rows) dbias_row<kHeld>(a.dbias_rows, at, nw, total[0], sums);
 }
 
-// 42 operations per element (78 us of all SIMDs for 67 M elements) beside five streams, two workgroups per CU: [16384, 4, 1024]
-// bfloat16, 688 MB in 170 us (4.0 TB/s).  At 6 waves per SIMD its span no longer fits the registers (219 us).
+// 54 operations per element (95 us of all SIMDs for 67 M elements) beside five streams, two workgroups per CU: [16384, 4, 1024]
+// bfloat16, 688 MB in 185 us (3.7 TB/s).  At 6 waves per SIMD its span no longer fits the registers (40 us slower).
 template <class T>
 __global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel(BackwardArgs<T> a, Chain ch) {
     __shared__ ChainSpace<sizeof(T) == 4, 1> mem;
@@ -1007,7 +1008,7 @@ __global__ __launch_bounds__(64 * kChainWaves, 4) void glr_backward_chain_kernel
     if (a.dbias_rows) dbias_row<kChainWaves>(a.dbias_rows + (int64_t)d.batch * a.C, d.at, kChainWaves, total[0], sums);
 }
 
-// One step: every thread V channels, nothing to share.  [2048, 256] float32, 10.5 MB in 4.1 us, of which a launch of nothing takes 3.5.
+// One step: every thread V channels, nothing to share.  [2048, 256] float32, 10.5 MB in 4 us, of which a launch of nothing takes 3.5.
 template <class T, int V>
 __global__ __launch_bounds__(256) void glr_step_kernel(Seq<const T> f, Seq<const T> x, const float *__restrict__ bias, Seq<const uint8_t> resets,
                                                        const float *h0, unsigned C, unsigned H, Seq<T> y, float *h_last, float *__restrict__ saved) {
@@ -1099,11 +1100,12 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
 
 // How a call is cut: tiles of 64 V columns (V channels per lane), and the time axis held by one workgroup per tile (up to 256 steps),
 // passed along a chain of workgroups, or, back over many 16-bit columns, walked by one wave per tile, which has no exchange and keeps
-// 3 waves per SIMD loading.  Measured, us forward / backward:
-//   [128, 1024 x 64] float32: held 21 / 39, chain 26 / 41, walked 26 / 40; bfloat16 [128, 768 x 64]: 14 / 30, 20 / 35, 17 / 31
-//   [2048, 384 x 64] float32: chain 116 / 202, walked 233 / 375; 1024 x 64: 314 / 531, 330 / 539
-//   [2048, E, H] bfloat16, 768 x 64 columns: chain 122 / 264, walked 223 / 316; 1536 x 64: 240 / 512, 270 / 474; 4096 x 64: 641 / 1312,
-//   688 / 1290; [128, 1536 x 64]: held 18 / 37, walked 22 / 37; [256, 8192 x 64]: 165 / 354, 172 / 313
+// 3 waves per SIMD loading.  Measured, us:
+//   held and chain, forward / backward: [128, 1024 x 64] float32 20 / 36 and 23 / 39, [128, 768 x 64] bfloat16 12 / 23 and 16 / 26,
+//   [256, 1279 x 64] 32 / 61 and 31 / 59
+//   bfloat16 backward, held and walked: [128, E, H] of 768 x 64 columns 23 and 31, 1279 x 64: 32 and 37, 1536 x 64: 37 and 40,
+//   3072 x 64: 70 and 64, 8192 x 64: 201 and 193; [256, E, H] 1279 x 64: 61 and 62, 1536 x 64: 72 and 67, 4096 x 64: 200 and 191
+//   chain and walked: [2048, E, H] 768 x 64: 275 and 370, 1279 x 64: 449 and 446, 1536 x 64: 542 and 488, 4096 x 64: 1415 and 1380
 struct Cut {
     enum { kHold, kWalk, kChain } how;
     int V, env_tiles, batches, words;        // words of a run

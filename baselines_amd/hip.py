@@ -231,7 +231,8 @@ def glr_forward(f, x, h0=None, resets=None, bias=None, y=None, h_last=None, want
     and ``h0`` [E, H] float32 (default zeros).  Returns (y, h_last, saved): y in x's type, the last state [E, H] in float32 and,
     with ``want_saved``, what :func:`glr_backward` needs.  An infinite state passes every gate, also one of minus infinity.
     ``y`` and ``h_last`` may be brought; they must not overlap each other or the inputs.  Beyond 256 steps workgroups hand the
-    state to each other; should one ever give up waiting, :func:`take_faults` says so."""
+    state to each other; should one ever give up waiting, :func:`take_faults` says so.  Nothing is recorded for automatic
+    differentiation, whatever the inputs require: :func:`glr_backward` takes the gradients."""
     if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _GLR_TYPES:
         raise TypeError("x must be a float32, bfloat16 or float16 tensor [T, E, H]")
     shape, dt = x.shape, x.dtype

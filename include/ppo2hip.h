@@ -500,7 +500,9 @@ typedef struct ppo2hip_seq {
  *           which ppo2hip_glr_backward recomputes the others from
  *   workspace : ppo2hip_glr_forward_workspace_bytes(...) bytes (may be 0), 16-byte aligned, for this call alone until it has run;
  *               nothing is kept in it from call to call
- * E*H may reach 2^31 - 1 and H 2^26 - 1 (more than 256 steps: E*H below 2^30).  T = 0 copies h0 to h_last.
+ * E*H may reach 2^31 - 1 and H 2^26 - 1, beyond 256 steps E*H 2^30 - 1, as far as a launch's 2^32 threads go; what does not fit is
+ * refused.  They are E*H for each 16 steps begun (beyond 256 steps: 8 E*H for each 128), half as many forward in 16 bits when H is
+ * even, and E*H in all for a single step and for the gradients of 81857 and more 16-bit columns.  T = 0 copies h0 to h_last.
  * Up to 256 steps one launch; more: a small launch that clears the workspace and one whose workgroups hand the state on.  Their waits
  * are bounded: one that gives up raises PPO2HIP_FAULT_GRID_SYNC (ppo2hip_take_faults) and leaves NaN behind. */
 int64_t ppo2hip_glr_saved_floats(int T, int E, int H);
