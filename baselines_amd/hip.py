@@ -1108,11 +1108,11 @@ class AdamWPlan:
 
 def adamw_step(plan, grads, lr, t, beta1=0.9, beta2=0.999, epsilon=1e-8, weight_decay=0.01, max_grad_norm=0.0, grad_scale=1.0):
     """One AdamW step of every tensor of ``plan``: step count ``t`` (1 for the first), gradients in list order (contiguous, in
-    their tensors' shapes or flat; None leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by the norm over all of them when
-    ``max_grad_norm`` > 0.  Bias-corrected roots next to ``epsilon`` and decay apart from the gradient: unlike :func:`adam_step`,
-    which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  Gradients must not share memory with the parameters or moments.  A
-    plan's steps go one after the other, also those of HIP graphs that captured them (they share its moments and workspace); a
-    captured call keeps ``lr``, ``t`` and the gradients' addresses."""
+    their tensors' shapes or flat; None leaves a tensor and its moments as they are), scaled by ``grad_scale``, then clipped by
+    the norm over all of them when ``max_grad_norm`` > 0.  Bias-corrected roots next to ``epsilon`` and decay apart from the
+    gradient: unlike :func:`adam_step`, which follows MpiAdam (baselines/common/mpi_adam.py:30-35).  Gradients must not share
+    memory with the parameters or moments.  A plan's steps go one after the other, also those of HIP graphs that captured them
+    (they share its moments and workspace); a captured call keeps ``lr``, ``t`` and the gradients' addresses."""
     gpu = plan._gpu
     if gpu != torch._C._cuda_getDevice():
         with torch.cuda.device(plan.device):
