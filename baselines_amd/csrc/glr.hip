@@ -1104,7 +1104,7 @@ extern "C" int64_t ppo2hip_glr_saved_floats(int T, int E, int H) {
 //   held and chain, forward / backward: [128, 1024 x 64] float32 20 / 36 and 23 / 39, [128, 768 x 64] bfloat16 12 / 23 and 16 / 26,
 //   [256, 1279 x 64] 32 / 61 and 31 / 59
 //   bfloat16 backward, held and walked: [128, E, H] of 768 x 64 columns 23 and 31, 1279 x 64: 32 and 37, 1536 x 64: 37 and 40,
-//   3072 x 64: 70 and 64, 8192 x 64: 201 and 193; [256, E, H] 1279 x 64: 61 and 62, 1536 x 64: 72 and 67, 4096 x 64: 200 and 191
+//   2048 x 64: 45 and 48, 8192 x 64: 201 and 193; [256, E, H] 1279 x 64: 61 and 62, 1536 x 64: 72 and 67, 4096 x 64: 200 and 191
 //   chain and walked: [2048, E, H] 768 x 64: 275 and 370, 1279 x 64: 449 and 446, 1536 x 64: 542 and 488, 4096 x 64: 1415 and 1380
 struct Cut {
     enum { kHold, kWalk, kChain } how;
